@@ -289,6 +289,54 @@ rcu_status rcu_window_attention(rcu_device* dev, const rcu_tensor* q, const rcu_
 rcu_status rcu_grouped_attention(rcu_device* dev, const rcu_tensor* q, const rcu_tensor* kv, const rcu_tensor* sink, uint32_t kv_heads, uint32_t vdim,
                                  uint32_t window, uint32_t chunk, uint32_t position, float scale, rcu_tensor* dst);
 
+/* ------------------------------------------------------------------ paged caches of many sequences
+ * No counterpart in the reference, whose caches hold one sequence in contiguous rows (ratchet-nn/src/kv_cache.rs:11-18).  Keys and values
+ * of many sequences lie in pages of `page_rows` rows (a power of two, 16 to 1024): row r of sequence s is row r mod page_rows of page
+ * table[s][r / page_rows].  A call brings new tokens of every sequence, one or many, back to back: tokens starts[s] .. starts[s + 1] - 1 are the
+ * last ones of the lengths[s] rows that sequence s has with them (none, where the two starts are equal).  Tokens before starts[0] and from
+ * starts[sequences] on belong to no sequence: nothing is read for them, and what the output has there stays.  The four index tensors are read
+ * on the device, so that a captured call can be replayed over new ones; entries of the table behind a sequence's last row are not read.  A start,
+ * length or page outside its tensor raises RCU_ERR_BOUNDS at the next rcu_sync / rcu_d2h, as does a length below the tokens brought; such
+ * entries are clamped, and outputs of the call are then not to be relied on.
+ * Pages may be shared by sequences (a common prompt) as long as nobody writes to them.
+ * dim and vdim are multiples of 8, at most 256; keys, values, and what is read or written with them, have one dtype, F32, F16 or BF16. */
+typedef struct {
+    rcu_tensor keys;      /* [pages, kv_heads, page_rows, dim] */
+    rcu_tensor values;    /* [pages, kv_heads, page_rows, vdim] */
+    rcu_tensor table;     /* I32 [sequences, max_pages] */
+    rcu_tensor starts;    /* I32 [sequences + 1] */
+    rcu_tensor lengths;   /* I32 [sequences] */
+    rcu_tensor mass;      /* F32 [sequences, kv_heads, max_pages * page_rows]: the attention weight that every row has received; data NULL: not kept */
+} rcu_paged;
+/* Rotation by positions that are given per token, on up to four axes (a text has one; images and video turn groups of pairs by time, row
+ * and column): x [tokens, W] holds heads of dst's dim from column x_col on, dst [tokens, heads, dim] has x's dtype.  freqs F32 [2, pairs] (value and
+ * remainder), positions I32 [axes, tokens]; the first sections[0] pairs go by axis 0, the next sections[1] by axis 1, and so on (host array; the
+ * sections add up to the pairs).  Pair i is features (first + 2i, first + 2i + 1), or with `halves` (first + i, first + pairs + i).  cos and sin, times
+ * `magnitude`, of angles evaluated in 64 bits.  dst may be x itself where x holds nothing else; any other overlap is refused. */
+rcu_status rcu_rotary_axes(rcu_device* dev, const rcu_tensor* x, uint32_t x_col, uint32_t first, const rcu_tensor* freqs, float magnitude,
+                           const rcu_tensor* positions, const uint32_t* sections, int halves, rcu_tensor* dst);
+/* Keys (columns [k_col, k_col + kv_heads * dim) of the rows k) and values (of the rows v, which may be k) of the new tokens into their pages; the
+ * rows' mass, where it is kept, becomes zero.  Two tokens of one call must not go to the same row of a page. */
+rcu_status rcu_paged_append(rcu_device* dev, const rcu_tensor* k, uint32_t k_col, const rcu_tensor* v, uint32_t v_col, const rcu_paged* cache);
+/* Softmax attention of the new tokens (already appended) over their sequences' pages: q [tokens, H, dim], query head h reads key / value head
+ * h / (H / kv_heads).  The token at row r of its sequence sees rows j <= r, with window > 0 only those with j > r - window or j < first.
+ * sink F32 [H] (nullable): exp(sink[h]) joins the denominator.  dst [tokens, H * vdim].  Where mass is kept, every row's sum grows by the
+ * weights (shares of the denominator) that the group's heads and the new tokens give it; sums are formed in the same order in every call.
+ * scratch (nullable): device memory of rcu_paged_attention_scratch bytes, any dtype; NULL takes it from the pool, which is refused while the
+ * stream is being captured.  Calls that share a scratch must not overlap. */
+rcu_status rcu_paged_attention(rcu_device* dev, const rcu_tensor* q, const rcu_paged* cache, const rcu_tensor* sink, uint32_t window, uint32_t first,
+                               float scale, const rcu_tensor* scratch, rcu_tensor* dst);
+uint64_t rcu_paged_attention_scratch(rcu_device* dev, const rcu_tensor* q, const rcu_paged* cache);
+/* Every sequence of more than `keep` rows is cut down to that many, each kv head by itself: its first `first` rows, its last `recent` rows and, of
+ * those between, the ones with the largest mass (of equal ones the lower rows; NaN counts as the least), in their order, become rows 0 .. keep - 1 of
+ * the sequence in `into`, with their mass; into->lengths receives the new lengths.  Shorter sequences go over whole.  `into` has the same sequences,
+ * kv heads, dims, page size and dtype, room for min(keep, its sequence's rows) in its table, and starts are not read.  It may name the same pages
+ * in the same places (in place: its table and mass may be cache's own; its lengths may not), or pages that no sequence of `cache` reads; a page that
+ * is written belongs to one sequence.  scratch as in rcu_paged_attention, of rcu_paged_evict_scratch bytes. */
+rcu_status rcu_paged_evict(rcu_device* dev, const rcu_paged* cache, const rcu_paged* into, uint32_t keep, uint32_t first, uint32_t recent,
+                           const rcu_tensor* scratch);
+uint64_t rcu_paged_evict_scratch(rcu_device* dev, const rcu_paged* cache, uint32_t keep);
+
 /* ------------------------------------------------------------------ lazy tensor graph (tensor.rs)
  * rcu_lazy is ratchet-core's `Tensor` (tensor.rs:45-47): a reference-counted node of a lazy DAG.
  * Builders validate their arguments and compute the output view exactly when the reference's
@@ -357,6 +405,19 @@ rcu_status rcu_lazy_latent_append(rcu_lazy* x, uint32_t x_col, rcu_lazy* scale, 
                                   rcu_lazy* ring, uint32_t rows, rcu_lazy** out);
 rcu_status rcu_lazy_window_attention(rcu_lazy* q, rcu_lazy* kv, rcu_lazy* shared, uint32_t shared_col, uint32_t vdim, uint32_t window, float scale,
                                      rcu_lazy** out);
+
+/* Paged caches as nodes.  keys, values, table, starts, mass (nullable) are resolved tensors; what a node writes to them is a side effect.
+ * rcu_lazy_paged_append and rcu_lazy_paged_evict give the sequences' lengths as they are behind the node, I32 [sequences]: who reads the
+ * cache after them takes that tensor as its `lengths`. */
+rcu_status rcu_lazy_rotary_axes(rcu_lazy* x, uint32_t x_col, uint32_t heads, uint32_t dim, uint32_t first, rcu_lazy* freqs, float magnitude,
+                                rcu_lazy* positions, const uint32_t* sections, int halves, rcu_lazy** out);
+rcu_status rcu_lazy_paged_append(rcu_lazy* k, uint32_t k_col, rcu_lazy* v, uint32_t v_col, rcu_lazy* keys, rcu_lazy* values, rcu_lazy* table,
+                                 rcu_lazy* starts, rcu_lazy* lengths, rcu_lazy* mass, rcu_lazy** out);
+rcu_status rcu_lazy_paged_attention(rcu_lazy* q, rcu_lazy* keys, rcu_lazy* values, rcu_lazy* table, rcu_lazy* starts, rcu_lazy* lengths,
+                                    rcu_lazy* mass, rcu_lazy* sink, uint32_t window, uint32_t first, float scale, rcu_lazy** out);
+rcu_status rcu_lazy_paged_evict(rcu_lazy* keys, rcu_lazy* values, rcu_lazy* table, rcu_lazy* lengths, rcu_lazy* mass, rcu_lazy* into_keys,
+                                rcu_lazy* into_values, rcu_lazy* into_table, rcu_lazy* into_mass, uint32_t keep, uint32_t first, uint32_t recent,
+                                rcu_lazy** out);
 
 /* Tensor::id (tensor.rs:100-104): process-wide unique, increasing with creation. */
 uint64_t rcu_lazy_id(const rcu_lazy* t);

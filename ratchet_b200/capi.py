@@ -87,7 +87,12 @@ class rcu_stack_run(C.Structure):
                                            "kv_norm", "sink", "uq", "ukv", "freqs", "decay", "out", "out_bias", "gate_up", "down", "state")])
 
 
+class rcu_paged(C.Structure):
+    _fields_ = [(n, rcu_tensor) for n in ("keys", "values", "table", "starts", "lengths", "mass")]
+
+
 _T = C.POINTER(rcu_tensor)
+_P = C.POINTER(rcu_paged)
 _DEV = C.c_void_p
 _LZ = C.c_void_p
 _u64p = C.POINTER(C.c_uint64)
@@ -148,6 +153,12 @@ SIGNATURES = {
     "rcu_norm_rotary": (C.c_int, [_DEV, _T, C.c_uint32, _T, C.c_float, _T, _T]),
     "rcu_kv_append": (C.c_int, [_DEV, _T, C.c_uint32, C.c_uint32, _T, C.c_float, _T, C.c_uint32, C.c_uint32, _T, _T]),
     "rcu_grouped_attention": (C.c_int, [_DEV, _T, _T, _T] + [C.c_uint32] * 5 + [C.c_float, _T]),
+    "rcu_rotary_axes": (C.c_int, [_DEV, _T, C.c_uint32, C.c_uint32, _T, C.c_float, _T, _u32p, C.c_int, _T]),
+    "rcu_paged_append": (C.c_int, [_DEV, _T, C.c_uint32, _T, C.c_uint32, _P]),
+    "rcu_paged_attention": (C.c_int, [_DEV, _T, _P, _T, C.c_uint32, C.c_uint32, C.c_float, _T, _T]),
+    "rcu_paged_attention_scratch": (C.c_uint64, [_DEV, _T, _P]),
+    "rcu_paged_evict": (C.c_int, [_DEV, _P, _P, C.c_uint32, C.c_uint32, C.c_uint32, _T]),
+    "rcu_paged_evict_scratch": (C.c_uint64, [_DEV, _P, C.c_uint32]),
     "rcu_glu": (C.c_int, [_DEV, C.c_int, _T, _T]),
     "rcu_rotary_frequencies": (C.c_int, [C.c_uint32] + [C.c_double] * 5 + [C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     "rcu_rotary": (C.c_int, [_DEV, _T, C.c_uint32, _T, C.c_float, C.c_uint32, _T]),
@@ -190,6 +201,10 @@ SIGNATURES = {
     "rcu_lazy_glu": (C.c_int, [C.c_int, _LZ, C.POINTER(_LZ)]),
     "rcu_lazy_rotary": (C.c_int, [_LZ, C.c_uint32, _LZ, C.c_float, C.c_uint32, C.POINTER(_LZ)]),
     "rcu_lazy_lightning": (C.c_int, [_LZ, _LZ, _LZ, C.POINTER(_LZ)]),
+    "rcu_lazy_rotary_axes": (C.c_int, [_LZ] + [C.c_uint32] * 4 + [_LZ, C.c_float, _LZ, _u32p, C.c_int, C.POINTER(_LZ)]),
+    "rcu_lazy_paged_append": (C.c_int, [_LZ, C.c_uint32, _LZ, C.c_uint32] + [_LZ] * 6 + [C.POINTER(_LZ)]),
+    "rcu_lazy_paged_attention": (C.c_int, [_LZ] * 8 + [C.c_uint32, C.c_uint32, C.c_float, C.POINTER(_LZ)]),
+    "rcu_lazy_paged_evict": (C.c_int, [_LZ] * 9 + [C.c_uint32] * 3 + [C.POINTER(_LZ)]),
     "rcu_lazy_latent_append": (C.c_int, [_LZ, C.c_uint32, _LZ, C.c_float, _LZ, C.c_float, C.c_uint32, _LZ, C.c_uint32, C.POINTER(_LZ)]),
     "rcu_lazy_window_attention": (C.c_int, [_LZ, _LZ, _LZ, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float, C.POINTER(_LZ)]),
     "rcu_lazy_id": (C.c_uint64, [_LZ]),

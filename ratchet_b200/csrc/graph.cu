@@ -28,13 +28,16 @@
 #include "common.cuh"
 #include "half_chains.cuh"
 
+rcu_status rcu_paged_append_to(rcu_device* dev, const rcu_tensor* k, uint32_t k_col, const rcu_tensor* v, uint32_t v_col, const rcu_paged* cache, int* lengths_out);   // paged_cache.cu
+
 namespace {
 
 enum LazyKind {
     K_CONST = 0, K_VIEW, K_BINARY, K_UNARY, K_CAST, K_MATMUL, K_NORM, K_SOFTMAX, K_ROPE, K_CONCAT, K_SELECT,
     K_PERMUTE, K_SLICE, K_BROADCAST, K_CACHE, K_INDEX_WRITE, K_CONV,
     K_LINEAR, K_NORM_ROWS, K_GLU, K_ROTARY, K_LIGHTNING, K_LATENT_APPEND, K_WINDOW_ATTENTION,
-    K_STREAM_ROWS, K_POST_NORM, K_ROTARY_ANGLES, K_NORM_ROTARY, K_KV_APPEND, K_GROUPED_ATTENTION
+    K_STREAM_ROWS, K_POST_NORM, K_ROTARY_ANGLES, K_NORM_ROTARY, K_KV_APPEND, K_GROUPED_ATTENTION,
+    K_ROTARY_AXES, K_PAGED_APPEND, K_PAGED_ATTENTION, K_PAGED_EVICT
 };
 
 struct Storage {
@@ -267,6 +270,10 @@ const char* kind_name(int kind) {
         case K_NORM_ROTARY: return "norm_rotary";
         case K_KV_APPEND: return "kv_append";
         case K_GROUPED_ATTENTION: return "grouped_attention";
+        case K_ROTARY_AXES: return "rotary_axes";
+        case K_PAGED_APPEND: return "paged_append";
+        case K_PAGED_ATTENTION: return "paged_attention";
+        case K_PAGED_EVICT: return "paged_evict";
         default: return "other";
     }
 }
@@ -374,6 +381,27 @@ rcu_status run_node(rcu_lazy* n, void* converted) {
             rcu_tensor q = S(0), kv = S(1), sink;
             if (n->srcs.size() > 2) sink = S(2);
             return rcu_grouped_attention(dev, &q, &kv, n->srcs.size() > 2 ? &sink : nullptr, n->u[0], n->u[1], n->u[2], n->u[3], n->u[4], n->f[0], &dst);
+        }
+        case K_ROTARY_AXES: {
+            rcu_tensor x = S(0), fr = S(1), at = S(2);
+            uint32_t sections[4];
+            for (int i = 0; i < 4; ++i) sections[i] = (uint32_t)n->a[i];
+            return rcu_rotary_axes(dev, &x, n->u[0], n->u[1], &fr, n->f[0], &at, sections, n->flags[0], &dst);
+        }
+        case K_PAGED_APPEND: {      // k, v, keys, values, table, starts, lengths, [mass]
+            rcu_tensor k = S(0), v = S(1);
+            const rcu_paged c{S(2), S(3), S(4), S(5), S(6), n->srcs.size() > 7 ? S(7) : rcu_tensor{}};
+            return rcu_paged_append_to(dev, &k, n->u[0], &v, n->u[1], &c, (int*)dst.data);
+        }
+        case K_PAGED_ATTENTION: {   // q, keys, values, table, starts, lengths, [mass], [sink]
+            rcu_tensor q = S(0), sink;
+            const rcu_paged c{S(1), S(2), S(3), S(4), S(5), n->flags[0] ? S(6) : rcu_tensor{}};
+            if (n->flags[1]) sink = S(6 + n->flags[0]);
+            return rcu_paged_attention(dev, &q, &c, n->flags[1] ? &sink : nullptr, n->u[0], n->u[1], n->f[0], nullptr, &dst);
+        }
+        case K_PAGED_EVICT: {       // keys, values, table, lengths, mass, then the new keys, values, table, mass
+            const rcu_paged c{S(0), S(1), S(2), rcu_tensor{}, S(3), S(4)}, into{S(5), S(6), S(7), rcu_tensor{}, dst, S(8)};
+            return rcu_paged_evict(dev, &c, &into, n->u[0], n->u[1], n->u[2], nullptr);
         }
         default: return rcu_fail(dev, RCU_ERR_UNSUPPORTED, "resolve: node kind %d has no kernel", n->kind);
     }
@@ -1266,6 +1294,83 @@ rcu_status rcu_lazy_grouped_attention(rcu_lazy* q, rcu_lazy* kv, rcu_lazy* sink,
     n->u[3] = chunk;
     n->u[4] = position;
     n->f[0] = scale;
+    *out = n;
+    return RCU_OK;
+}
+
+rcu_status rcu_lazy_rotary_axes(rcu_lazy* x, uint32_t x_col, uint32_t heads, uint32_t dim, uint32_t first, rcu_lazy* freqs, float magnitude,
+                                rcu_lazy* positions, const uint32_t* sections, int halves, rcu_lazy** out) {
+    if (!x || !freqs || !positions || !sections || !out) return RCU_ERR_INVALID_ARG;
+    LAZY_REQUIRE(x->dev, x->rank == 2 && (uint64_t)x_col + (uint64_t)heads * dim <= x->shape[1], "rotary_axes: the heads lie outside the rows");
+    LAZY_REQUIRE(x->dev, freqs->rank == 2 && (uint64_t)first + 2 * freqs->shape[1] <= dim, "rotary_axes: the rotated features lie outside the head");
+    LAZY_REQUIRE(x->dev, positions->rank == 2 && positions->dt == RCU_I32 && positions->shape[0] >= 1 && positions->shape[0] <= 4 && positions->shape[1] == x->shape[0],
+                 "rotary_axes: positions are i32 [axes, tokens] of one to four axes");
+    uint64_t sum = 0;
+    for (uint64_t i = 0; i < positions->shape[0]; ++i) sum += sections[i];
+    LAZY_REQUIRE(x->dev, sum == freqs->shape[1], "rotary_axes: the sections hold %llu of %llu pairs", (unsigned long long)sum, (unsigned long long)freqs->shape[1]);
+    const uint64_t shape[3] = {x->shape[0], heads, dim};
+    rcu_lazy* n = new_node(x->dev, K_ROTARY_AXES, x->dt, 3, shape, {x, freqs, positions});
+    n->u[0] = x_col;
+    n->u[1] = first;
+    n->f[0] = magnitude;
+    n->flags[0] = halves != 0;
+    for (uint64_t i = 0; i < positions->shape[0]; ++i) n->a[i] = sections[i];
+    *out = n;
+    return RCU_OK;
+}
+
+// pages, tables and sums are there before a node that writes or reads them is built: their contents are not the graph's
+#define LAZY_RESOLVED(op, ...)                                                                                                   \
+    for (const rcu_lazy* t : {__VA_ARGS__})                                                                                      \
+    LAZY_REQUIRE(t ? t->dev : dev, t && t->resolved(), op ": pages, tables, starts and sums are resolved tensors")
+
+rcu_status rcu_lazy_paged_append(rcu_lazy* k, uint32_t k_col, rcu_lazy* v, uint32_t v_col, rcu_lazy* keys, rcu_lazy* values, rcu_lazy* table,
+                                 rcu_lazy* starts, rcu_lazy* lengths, rcu_lazy* mass, rcu_lazy** out) {
+    if (!k || !v || !keys || !values || !table || !starts || !lengths || !out) return RCU_ERR_INVALID_ARG;
+    rcu_device* dev = k->dev;
+    LAZY_RESOLVED("paged_append", keys, values, table, starts);
+    if (mass) LAZY_RESOLVED("paged_append", mass);
+    LAZY_REQUIRE(dev, keys->rank == 4 && values->rank == 4 && k->rank == 2 && v->rank == 2 && k->shape[0] == v->shape[0], "paged_append: rows k and v of the same tokens, pages of rank 4");
+    LAZY_REQUIRE(dev, (uint64_t)k_col + keys->shape[1] * keys->shape[3] <= k->shape[1] && (uint64_t)v_col + values->shape[1] * values->shape[3] <= v->shape[1],
+                 "paged_append: the heads lie outside the rows");
+    LAZY_REQUIRE(dev, lengths->dt == RCU_I32 && lengths->rank == 1 && table->rank == 2 && lengths->shape[0] == table->shape[0], "paged_append: lengths are i32 [sequences]");
+    rcu_lazy* n = new_node(dev, K_PAGED_APPEND, RCU_I32, 1, lengths->shape, {k, v, keys, values, table, starts, lengths, mass});
+    n->u[0] = k_col;
+    n->u[1] = v_col;
+    *out = n;
+    return RCU_OK;
+}
+
+rcu_status rcu_lazy_paged_attention(rcu_lazy* q, rcu_lazy* keys, rcu_lazy* values, rcu_lazy* table, rcu_lazy* starts, rcu_lazy* lengths,
+                                    rcu_lazy* mass, rcu_lazy* sink, uint32_t window, uint32_t first, float scale, rcu_lazy** out) {
+    if (!q || !keys || !values || !table || !starts || !lengths || !out) return RCU_ERR_INVALID_ARG;
+    rcu_device* dev = q->dev;
+    LAZY_RESOLVED("paged_attention", keys, values, table, starts);
+    if (mass) LAZY_RESOLVED("paged_attention", mass);
+    LAZY_REQUIRE(dev, q->rank == 3 && keys->rank == 4 && values->rank == 4 && q->shape[2] == keys->shape[3], "paged_attention: q is [tokens, heads, dim] of the pages' dim");
+    const uint64_t shape[2] = {q->shape[0], q->shape[1] * values->shape[3]};
+    rcu_lazy* n = new_node(dev, K_PAGED_ATTENTION, q->dt, 2, shape, {q, keys, values, table, starts, lengths, mass, sink});
+    n->flags[0] = mass != nullptr;
+    n->flags[1] = sink != nullptr;
+    n->u[0] = window;
+    n->u[1] = first;
+    n->f[0] = scale;
+    *out = n;
+    return RCU_OK;
+}
+
+rcu_status rcu_lazy_paged_evict(rcu_lazy* keys, rcu_lazy* values, rcu_lazy* table, rcu_lazy* lengths, rcu_lazy* mass, rcu_lazy* into_keys,
+                                rcu_lazy* into_values, rcu_lazy* into_table, rcu_lazy* into_mass, uint32_t keep, uint32_t first, uint32_t recent,
+                                rcu_lazy** out) {
+    if (!keys || !values || !table || !lengths || !mass || !into_keys || !into_values || !into_table || !into_mass || !out) return RCU_ERR_INVALID_ARG;
+    rcu_device* dev = keys->dev;
+    LAZY_RESOLVED("paged_evict", keys, values, table, mass, into_keys, into_values, into_table, into_mass);
+    LAZY_REQUIRE(dev, lengths->dt == RCU_I32 && lengths->rank == 1 && table->rank == 2 && lengths->shape[0] == table->shape[0], "paged_evict: lengths are i32 [sequences]");
+    LAZY_REQUIRE(dev, keep >= 1 && (uint64_t)first + recent <= keep, "paged_evict: %u first and %u recent rows of %u to keep", first, recent, keep);
+    rcu_lazy* n = new_node(dev, K_PAGED_EVICT, RCU_I32, 1, lengths->shape, {keys, values, table, lengths, mass, into_keys, into_values, into_table, into_mass});
+    n->u[0] = keep;
+    n->u[1] = first;
+    n->u[2] = recent;
     *out = n;
     return RCU_OK;
 }

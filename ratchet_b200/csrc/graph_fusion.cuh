@@ -560,11 +560,20 @@ struct Pass {
         if (!on) return;
         for (const rcu_lazy* t : o.nodes) {
             if (t->resolved()) continue;
-            const bool first = t->kind == K_CACHE || t->kind == K_INDEX_WRITE, third = t->kind == K_LIGHTNING, fourth = t->kind == K_LATENT_APPEND || t->kind == K_KV_APPEND;
-            if (!first && !third && !fourth) continue;
-            const rcu_lazy* w = viewed(t->srcs[first ? 0 : third ? 2 : 3]);
-            const char* begin = w->resolved() ? (const char*)w->storage->ptr : nullptr;
-            written.push_back(Written{w, begin, begin ? begin + w->nbytes() : nullptr});
+            auto writes = [&](size_t src) {
+                const rcu_lazy* w = viewed(t->srcs[src]);
+                const char* begin = w->resolved() ? (const char*)w->storage->ptr : nullptr;
+                written.push_back(Written{w, begin, begin ? begin + w->nbytes() : nullptr});
+            };
+            switch (t->kind) {
+                case K_CACHE: case K_INDEX_WRITE: writes(0); break;
+                case K_LIGHTNING: writes(2); break;
+                case K_LATENT_APPEND: case K_KV_APPEND: writes(3); break;
+                case K_PAGED_APPEND: writes(2); writes(3); if (t->srcs.size() > 7) writes(7); break;
+                case K_PAGED_ATTENTION: if (t->flags[0]) writes(6); break;
+                case K_PAGED_EVICT: writes(5); writes(6); writes(8); break;
+                default: break;
+            }
         }
         for (size_t i = o.nodes.size(); i-- > 0;) {
             rcu_lazy* t = o.nodes[i];

@@ -27,7 +27,7 @@ static PyTypeObject NodeType;
     X(release) X(retain) X(info) X(strong_count) X(binary) X(unary) X(cast) X(norm) X(softmax) X(rope) X(matmul) X(conv1d)  \
     X(view) X(slice) X(permute) X(broadcast) X(index_select) X(cache) X(linear) X(norm_rows) X(stream_rows) X(post_norm)    \
     X(bitcast) X(rotary_angles) X(norm_rotary) X(kv_append) X(grouped_attention) X(glu) X(rotary) X(lightning)              \
-    X(latent_append) X(window_attention)
+    X(latent_append) X(window_attention) X(rotary_axes) X(paged_append) X(paged_attention) X(paged_evict)
 #define X(name) static __typeof__(&rcu_lazy_##name) p_##name;
 FUNCTIONS(X)
 #undef X
@@ -405,6 +405,31 @@ METHOD(_grouped_attention) {    /* kv, sink, kv_heads, vdim, window, chunk, posi
     POSITIONAL("_grouped_attention", 8) NODE(0); NODE(1); WORD(2); WORD(3); WORD(4); WORD(5); WORD(6); REAL(7);
     DONE(p_grouped_attention(self->h, x0, x1, (uint32_t)w2, (uint32_t)w3, (uint32_t)w4, (uint32_t)w5, (uint32_t)w6, f7, &out));
 }
+METHOD(_rotary_axes) {  /* col, heads, dim, first, freqs, magnitude, positions, sections, halves */
+    POSITIONAL("_rotary_axes", 9) WORD(0); WORD(1); WORD(2); WORD(3); NODE(4); REAL(5); NODE(6); WORD(8);
+    uint64_t s[4];
+    uint32_t sections[4] = {0, 0, 0, 0};
+    Py_ssize_t axes;
+    rcu_tensor t;
+    memset(&t, 0, sizeof t);
+    if (!as_words(v[7], 0, s, 4, &axes)) return NULL;
+    if (x6) p_info(x6, &t);
+    if (axes > 4 || (x6 && (uint64_t)axes != t.shape[0])) return PyErr_Format(PyExc_ValueError, "rotary_axes: one section per axis, four at most");
+    for (Py_ssize_t i = 0; i < axes; ++i) sections[i] = (uint32_t)s[i];
+    DONE(p_rotary_axes(self->h, (uint32_t)w0, (uint32_t)w1, (uint32_t)w2, (uint32_t)w3, x4, f5, x6, sections, (int)w8, &out));
+}
+METHOD(_paged_append) {  /* col, v, v_col, keys, values, table, starts, lengths, mass */
+    POSITIONAL("_paged_append", 9) WORD(0); NODE(1); WORD(2); NODE(3); NODE(4); NODE(5); NODE(6); NODE(7); NODE(8);
+    DONE(p_paged_append(self->h, (uint32_t)w0, x1, (uint32_t)w2, x3, x4, x5, x6, x7, x8, &out));
+}
+METHOD(_paged_attention) {  /* keys, values, table, starts, lengths, mass, sink, window, first, scale */
+    POSITIONAL("_paged_attention", 10) NODE(0); NODE(1); NODE(2); NODE(3); NODE(4); NODE(5); NODE(6); WORD(7); WORD(8); REAL(9);
+    DONE(p_paged_attention(self->h, x0, x1, x2, x3, x4, x5, x6, (uint32_t)w7, (uint32_t)w8, f9, &out));
+}
+METHOD(_paged_evict) {  /* values, table, lengths, mass, into: keys, values, table, mass; keep, first, recent */
+    POSITIONAL("_paged_evict", 11) NODE(0); NODE(1); NODE(2); NODE(3); NODE(4); NODE(5); NODE(6); NODE(7); WORD(8); WORD(9); WORD(10);
+    DONE(p_paged_evict(self->h, x0, x1, x2, x3, x4, x5, x6, x7, (uint32_t)w8, (uint32_t)w9, (uint32_t)w10, &out));
+}
 
 #define FAST(fn) {#fn, (PyCFunction)(void (*)(void))node_##fn, METH_FASTCALL | METH_KEYWORDS, NULL}
 #define NOARGS(fn) {#fn, (PyCFunction)(void (*)(void))node_##fn, METH_NOARGS, NULL}
@@ -417,6 +442,7 @@ static PyMethodDef node_methods[] = {
     FAST(slice), FAST(view), FAST(broadcast_to), FAST(permute), FAST(cache), FAST(index_select),
     FAST(_linear), FAST(_norm_rows), FAST(stream_rows), FAST(post_norm), FAST(bitcast), FAST(_glu), FAST(_rotary), FAST(lightning),
     FAST(_latent_append), FAST(window_attention), FAST(rotary_angles), FAST(_norm_rotary), FAST(_kv_append), FAST(_grouped_attention),
+    FAST(_rotary_axes), FAST(_paged_append), FAST(_paged_attention), FAST(_paged_evict),
     {NULL, NULL, 0, NULL}};
 
 static PyMemberDef node_members[] = {{"dev", T_OBJECT, offsetof(Node, dev), READONLY, NULL}, {NULL, 0, 0, 0, NULL}};

@@ -1,0 +1,163 @@
+// Rotation of head features by positions that are given per token, on up to four axes (rcu_rotary_axes): what a batch of sequences at
+// different places needs, and models of images and video, whose pairs turn by time, row or column.
+//
+//   (u, v) <- m (u cos a - v sin a, v cos a + u sin a),  a = position[axis of the pair][token] * frequency[pair]
+//
+// Bound by memory: every row is read and written once.  A CTA takes a few tokens: it works out their angles once, in shared memory, and then
+// turns all their heads, sixteen bytes of a row per thread and step.  The angle is a product of doubles, brought into [-pi, pi] by doubles
+// (so positions of any size keep their low bits), and only there goes on in f32: sine and cosine of a reduced f32 are off by
+// 1.2e-7 at most, half a unit of f32, and cost a tenth of a double's.
+#include "lm_math.cuh"
+
+namespace {
+
+struct AxesArgs {
+    const float* freqs;
+    const int* positions;      // [axes, T]
+    int ends[4];               // pairs that go by axis 0, 0..1, 0..2, 0..3
+    long long T;
+    long long pitch;           // of x's rows
+    int H, D, first, pairs, halves;
+    float magnitude;
+};
+
+__device__ __forceinline__ float2 turn_of(const AxesArgs& a, long long t, int i) {
+    const int axis = (i >= a.ends[0]) + (i >= a.ends[1]) + (i >= a.ends[2]);
+    const double angle = (double)a.positions[axis * a.T + t] * ((double)a.freqs[i] + (double)a.freqs[a.pairs + i]);
+    const double turns = rint(angle * 0.15915494309189535);
+    // 2 pi as two doubles
+    const double r = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, angle));
+    float s, c;
+    sincosf((float)r, &s, &c);
+    return make_float2(c * a.magnitude, s * a.magnitude);
+}
+
+// V elements of 16 bytes (VEC), or one by one; TOK tokens per CTA
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) rotary_axes_kernel(const AxesArgs a, const T* x, T* out, int tokens) {
+    rcu_kernel_entry();
+    extern __shared__ float2 cs[];
+    const long long t0 = (long long)blockIdx.x * tokens;
+    const int n = (int)min((long long)tokens, a.T - t0);
+    for (int i = threadIdx.x; i < n * a.pairs; i += 256) cs[i] = turn_of(a, t0 + i / a.pairs, i % a.pairs);
+    __syncthreads();
+    const int lo = a.first, hi = a.first + 2 * a.pairs;
+    if constexpr (VEC) {
+        constexpr int V = 16 / (int)sizeof(T);
+        struct alignas(16) Vec { T v[V]; };
+        if (a.halves) {
+            // units of V pairs: V features of the first half and V of the second; then what is not turned
+            const int units = a.pairs / V, rest = (a.D - 2 * a.pairs) / V, per = units + rest;
+            for (int j = threadIdx.x; j < n * a.H * per; j += 256) {
+                const int t = j / (a.H * per), h = j / per % a.H, u = j % per;
+                const T* xr = x + (t0 + t) * a.pitch + (size_t)h * a.D;
+                T* o = out + ((t0 + t) * a.H + h) * (size_t)a.D;
+                if (u >= units) {
+                    int d = (u - units) * V;
+                    if (d >= lo) d += 2 * a.pairs;
+                    *reinterpret_cast<Vec*>(o + d) = *reinterpret_cast<const Vec*>(xr + d);
+                    continue;
+                }
+                const int d = lo + u * V;
+                const Vec p = *reinterpret_cast<const Vec*>(xr + d), q = *reinterpret_cast<const Vec*>(xr + d + a.pairs);
+                Vec y, z;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float2 w = cs[t * a.pairs + u * V + e];
+                    const float f = to_f32<T>(p.v[e]), g = to_f32<T>(q.v[e]);
+                    y.v[e] = from_f32<T>(f * w.x - g * w.y);
+                    z.v[e] = from_f32<T>(g * w.x + f * w.y);
+                }
+                *reinterpret_cast<Vec*>(o + d) = y;
+                *reinterpret_cast<Vec*>(o + d + a.pairs) = z;
+            }
+        } else {
+            const int per = a.D / V;
+            for (int j = threadIdx.x; j < n * a.H * per; j += 256) {
+                const int t = j / (a.H * per), h = j / per % a.H, d = j % per * V;
+                Vec p = *reinterpret_cast<const Vec*>(x + (t0 + t) * a.pitch + (size_t)h * a.D + d);
+                if (d >= lo && d < hi) {
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        const float2 w = cs[t * a.pairs + (d - lo + e) / 2];
+                        const float f = to_f32<T>(p.v[e]), g = to_f32<T>(p.v[e + 1]);
+                        p.v[e] = from_f32<T>(f * w.x - g * w.y);
+                        p.v[e + 1] = from_f32<T>(g * w.x + f * w.y);
+                    }
+                }
+                *reinterpret_cast<Vec*>(out + ((t0 + t) * a.H + h) * (size_t)a.D + d) = p;
+            }
+        }
+    } else {
+        const int rest = a.D - 2 * a.pairs, per = a.pairs + rest;
+        for (int j = threadIdx.x; j < n * a.H * per; j += 256) {
+            const int t = j / (a.H * per), h = j / per % a.H, u = j % per;
+            const T* xr = x + (t0 + t) * a.pitch + (size_t)h * a.D;
+            T* o = out + ((t0 + t) * a.H + h) * (size_t)a.D;
+            if (u >= a.pairs) {
+                int d = u - a.pairs;
+                if (d >= lo) d += 2 * a.pairs;
+                o[d] = xr[d];
+                continue;
+            }
+            const int d = lo + (a.halves ? u : 2 * u), e = d + (a.halves ? a.pairs : 1);
+            const float2 w = cs[t * a.pairs + u];
+            const float f = to_f32<T>(xr[d]), g = to_f32<T>(xr[e]);
+            o[d] = from_f32<T>(f * w.x - g * w.y);
+            o[e] = from_f32<T>(g * w.x + f * w.y);
+        }
+    }
+}
+
+template <class T> void launch_axes(rcu_device* dev, const AxesArgs& a, const void* x, void* out) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const bool vec = a.D % V == 0 && a.first % V == 0 && (a.halves ? a.pairs : 2 * a.pairs) % V == 0 && a.pitch % V == 0 &&
+                     ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    // enough work for a CTA's threads, as long as every SM gets some and the angles take 16 KB at most
+    int tokens = 1;
+    while (tokens < 8 && (long long)tokens * a.H * a.D < 8 * 256 * V && a.T / (2 * tokens) >= 2 * dev->sm_count && 2 * tokens * a.pairs <= 2048) tokens *= 2;
+    const unsigned grid = (unsigned)((a.T + tokens - 1) / tokens);
+    const size_t smem = (size_t)tokens * a.pairs * sizeof(float2);
+    if (vec) rcu_launch(dev, rotary_axes_kernel<T, true>, grid, 256, smem, a, (const T*)x, (T*)out, tokens);
+    else rcu_launch(dev, rotary_axes_kernel<T, false>, grid, 256, smem, a, (const T*)x, (T*)out, tokens);
+}
+
+}  // namespace
+
+extern "C" {
+
+rcu_status rcu_rotary_axes(rcu_device* dev, const rcu_tensor* x, uint32_t x_col, uint32_t first, const rcu_tensor* freqs, float magnitude,
+                           const rcu_tensor* positions, const uint32_t* sections, int halves, rcu_tensor* dst) {
+    if (!dev) return RCU_ERR_INVALID_ARG;
+    RCU_REQUIRE(dev, t_valid(x) && t_valid(freqs) && t_valid(positions) && sections && t_valid(dst), "rotary_axes: invalid tensor descriptor");
+    RCU_REQUIRE(dev, x->rank == 2 && dst->rank == 3 && x->dt == dst->dt && dt_is_float(x->dt) && dst->shape[0] == x->shape[0],
+                "rotary_axes: float rows x [tokens, width] and dst [tokens, heads, dim] of one dtype");
+    RCU_REQUIRE(dev, freqs->dt == RCU_F32 && freqs->rank == 2 && freqs->shape[0] == 2, "rotary_axes: the frequency table is f32 [2, pairs]");
+    const uint64_t T = x->shape[0], W = x->shape[1], H = dst->shape[1], D = dst->shape[2], pairs = freqs->shape[1];
+    RCU_REQUIRE(dev, positions->dt == RCU_I32 && positions->rank == 2 && positions->shape[0] >= 1 && positions->shape[0] <= 4 && positions->shape[1] == T,
+                "rotary_axes: positions are i32 [axes, tokens] of one to four axes");
+    RCU_REQUIRE(dev, H <= (1u << 20) && D <= (1u << 20) && H * D <= W && x_col <= W - H * D && W <= (1ull << 31), "rotary_axes: the heads lie outside the rows");
+    RCU_REQUIRE(dev, pairs <= 2048 && (uint64_t)first + 2 * pairs <= D && T < (1ull << 31) / 4, "rotary_axes: the rotated features lie outside the head");
+    AxesArgs a{(const float*)freqs->data, (const int*)positions->data, {}, (long long)T, (long long)W, (int)H, (int)D, (int)first, (int)pairs, halves != 0, magnitude};
+    uint64_t sum = 0;
+    for (int i = 0; i < 4; ++i) {
+        if ((uint64_t)i < positions->shape[0]) sum += sections[i];
+        a.ends[i] = (int)(sum < pairs ? sum : pairs);
+    }
+    RCU_REQUIRE(dev, sum == pairs, "rotary_axes: the sections hold %llu of %llu pairs", (unsigned long long)sum, (unsigned long long)pairs);
+    const size_t e = dt_esize(x->dt);
+    const char *xb = (const char*)x->data, *xe = xb + T * W * e, *ob = (const char*)dst->data, *oe = ob + T * H * D * e;
+    RCU_REQUIRE(dev, ob >= xe || oe <= xb || (ob == xb && W == H * D), "rotary_axes: dst overlaps rows of x that hold more than the heads");
+    if (T == 0 || H * D == 0) return RCU_OK;
+    // a wider index than an int holds is left out rather than wrapped: eight tokens' units per CTA
+    RCU_REQUIRE(dev, 8 * H * D < (1ull << 31), "rotary_axes: rows of %llu features", (unsigned long long)(H * D));
+    DevGuard g(dev->ordinal);
+    const void* xp = xb + (size_t)x_col * e;
+    if (x->dt == RCU_F32) launch_axes<float>(dev, a, xp, dst->data);
+    else if (x->dt == RCU_F16) launch_axes<__half>(dev, a, xp, dst->data);
+    else launch_axes<__nv_bfloat16>(dev, a, xp, dst->data);
+    RCU_LAUNCH_CHECK(dev);
+    return RCU_OK;
+}
+
+}  // extern "C"

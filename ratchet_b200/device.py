@@ -72,6 +72,17 @@ class Buffer:
             pass
 
 
+class PagedCache:
+    """``rcu_paged`` over device buffers: pages of keys and values [pages, kv_heads, page_rows, features], the table I32 [sequences, max_pages],
+    starts I32 [sequences + 1] of a call's new tokens, lengths I32 [sequences] with them, and (optional) the attention weight F32
+    [sequences, kv_heads, max_pages * page_rows] that every row has received.  A cache that evictions only write to needs no starts."""
+
+    def __init__(self, keys: Buffer, values: Buffer, table: Buffer, lengths: Buffer, starts: Optional[Buffer] = None, mass: Optional[Buffer] = None):
+        self.keys, self.values, self.table, self.starts, self.lengths, self.mass = keys, values, table, starts, lengths, mass
+        self.struct = capi.rcu_paged(*(b.desc() if b is not None else capi.rcu_tensor() for b in (keys, values, table, starts, lengths, mass)))
+        self.ref = C.byref(self.struct)
+
+
 class Device:
     """One CUDA device + stream + caching allocator (``rcu_device``)."""
 
@@ -406,3 +417,34 @@ class Device:
         self.check(self._lib.rcu_window_attention(self.handle, self._ref(q), self._ref(kv), self._ref(shared), shared_col, vdim, window, scale,
                                                   self._ref(out)))
         return out
+
+    # ------------------------------------------------------------------ paged caches of many sequences
+    def rotary_axes(self, x: Buffer, heads: int, dim: int, freqs: Buffer, positions: Buffer, sections: Sequence[int], magnitude: float = 1.0, col: int = 0,
+                    first: int = 0, halves: bool = False, out: Optional[Buffer] = None) -> Buffer:
+        if len(sections) != positions.shape[0]:
+            raise RatchetCudaError(capi.ERR_INVALID_ARG, f"rotary_axes: {len(sections)} sections for {positions.shape[0]} axes")
+        out = out or self.empty(x.dt, (x.shape[0], heads, dim))
+        self.check(self._lib.rcu_rotary_axes(self.handle, self._ref(x), col, first, self._ref(freqs), magnitude, self._ref(positions),
+                                             (C.c_uint32 * len(sections))(*sections), int(halves), self._ref(out)))
+        return out
+
+    def paged_append(self, k: Buffer, v: Buffer, cache: PagedCache, k_col: int = 0, v_col: int = 0) -> None:
+        self.check(self._lib.rcu_paged_append(self.handle, self._ref(k), k_col, self._ref(v), v_col, cache.ref))
+
+    def paged_attention_scratch(self, q: Buffer, cache: PagedCache) -> int:
+        """Bytes of the scratch that paged_attention takes (it must be given one while a stream is captured)."""
+        return self._lib.rcu_paged_attention_scratch(self.handle, self._ref(q), cache.ref)
+
+    def paged_attention(self, q: Buffer, cache: PagedCache, scale: float, sink: Optional[Buffer] = None, window: int = 0, first: int = 0,
+                        scratch: Optional[Buffer] = None, out: Optional[Buffer] = None) -> Buffer:
+        out = out or self.empty(q.dt, (q.shape[0], q.shape[1] * cache.values.shape[3]))
+        self.check(self._lib.rcu_paged_attention(self.handle, self._ref(q), cache.ref, self._ref(sink), window, first, scale, self._ref(scratch),
+                                                 self._ref(out)))
+        return out
+
+    def paged_evict_scratch(self, cache: PagedCache, keep: int) -> int:
+        return self._lib.rcu_paged_evict_scratch(self.handle, cache.ref, keep)
+
+    def paged_evict(self, cache: PagedCache, into: PagedCache, keep: int, first: int = 0, recent: int = 0, scratch: Optional[Buffer] = None) -> None:
+        """At most `keep` rows per sequence and kv head into `into`'s pages: the first ones, the recent ones and the heaviest between."""
+        self.check(self._lib.rcu_paged_evict(self.handle, cache.ref, into.ref, keep, first, recent, self._ref(scratch)))

@@ -171,3 +171,20 @@ class SequenceState:
                     n *= s
                 t.dev.check(t.dev._lib.rcu_memset(t.dev.handle, t.data_ptr(), 0, n))
         self.position = 0
+
+
+class PagedState:
+    """Graph tensors of a paged cache: pages of keys and values [pages, kv_heads, page_rows, features], the table I32 [sequences, max_pages], starts
+    I32 [sequences + 1] of a step's new tokens, lengths I32 [sequences] with them, and (optional) the attention weight F32 [sequences,
+    kv_heads, max_pages * page_rows] that every row has received."""
+
+    def __init__(self, keys, values, table, starts, lengths, mass=None):
+        self.keys, self.values, self.table, self.starts, self.lengths, self.mass = keys, values, table, starts, lengths, mass
+
+    def after(self, lengths) -> "PagedState":
+        """The same pages behind a node that wrote them: `lengths` is that node's output."""
+        return PagedState(self.keys, self.values, self.table, self.starts, lengths, self.mass)
+
+    def evict(self, into: "PagedState", keep: int, first: int = 0, recent: int = 0) -> "PagedState":
+        """At most `keep` rows per sequence and kv head, in `into`'s pages: the first ones, the recent ones and the heaviest between."""
+        return into.after(self.keys._paged_evict(self.values, self.table, self.lengths, self.mass, into.keys, into.values, into.table, into.mass, keep, first, recent))

@@ -157,6 +157,20 @@ class Tensor(Node):
         of `chunk` positions, or everything before."""
         return self._grouped_attention(kv, sink, kv_heads, vdim, window, chunk, position, scale)
 
+    # ------------------------------------------------------------------ paged caches (nn.PagedState)
+    def rotary_axes(self, heads: int, dim: int, freqs: "Tensor", positions: "Tensor", sections: Sequence[int], magnitude: float = 1.0, col: int = 0,
+                    first: int = 0, halves: bool = False) -> "Tensor":
+        """Rotation of heads in columns [col, col + heads * dim) by positions I32 [axes, tokens]; sections[a] pairs go by axis a: [tokens, heads, dim]."""
+        return self._rotary_axes(col, heads, dim, first, freqs, magnitude, positions, sections, halves)
+
+    def paged_append(self, v: "Tensor", cache, col: int = 0, v_col: int = 0):
+        """Keys in these rows and values in the rows v into their pages; the cache as who comes after it sees it."""
+        return cache.after(self._paged_append(col, v, v_col, cache.keys, cache.values, cache.table, cache.starts, cache.lengths, cache.mass))
+
+    def paged_attention(self, cache, scale: float, sink: Optional["Tensor"] = None, window: int = 0, first: int = 0) -> "Tensor":
+        """Softmax attention of these new tokens [tokens, heads, dim] over their sequences' pages; rows' sums grow where the cache keeps them."""
+        return self._paged_attention(cache.keys, cache.values, cache.table, cache.starts, cache.lengths, cache.mass, sink, window, first, scale)
+
     # ------------------------------------------------------------------ execution
     def resolve(self) -> "Tensor":
         """Tensor::resolve (tensor.rs:861-863). Asynchronous; ``to_numpy`` / ``Device.sync`` wait."""

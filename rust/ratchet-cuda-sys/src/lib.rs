@@ -84,6 +84,18 @@ pub struct rcu_tensor {
     pub data: *mut c_void,
 }
 
+/// Pages of many sequences' keys and values, with what names their rows.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct rcu_paged {
+    pub keys: rcu_tensor,
+    pub values: rcu_tensor,
+    pub table: rcu_tensor,
+    pub starts: rcu_tensor,
+    pub lengths: rcu_tensor,
+    pub mass: rcu_tensor,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
 pub struct rcu_resolve_stats {
@@ -275,6 +287,16 @@ extern "C" {
     pub fn rcu_grouped_attention(
         dev: *mut rcu_device, q: *const rcu_tensor, kv: *const rcu_tensor, sink: *const rcu_tensor, kv_heads: u32, vdim: u32, window: u32, chunk: u32, position: u32, scale: f32, dst: *mut rcu_tensor,
     ) -> rcu_status;
+    pub fn rcu_rotary_axes(
+        dev: *mut rcu_device, x: *const rcu_tensor, x_col: u32, first: u32, freqs: *const rcu_tensor, magnitude: f32, positions: *const rcu_tensor, sections: *const u32, halves: c_int, dst: *mut rcu_tensor,
+    ) -> rcu_status;
+    pub fn rcu_paged_append(dev: *mut rcu_device, k: *const rcu_tensor, k_col: u32, v: *const rcu_tensor, v_col: u32, cache: *const rcu_paged) -> rcu_status;
+    pub fn rcu_paged_attention(
+        dev: *mut rcu_device, q: *const rcu_tensor, cache: *const rcu_paged, sink: *const rcu_tensor, window: u32, first: u32, scale: f32, scratch: *const rcu_tensor, dst: *mut rcu_tensor,
+    ) -> rcu_status;
+    pub fn rcu_paged_attention_scratch(dev: *mut rcu_device, q: *const rcu_tensor, cache: *const rcu_paged) -> u64;
+    pub fn rcu_paged_evict(dev: *mut rcu_device, cache: *const rcu_paged, into: *const rcu_paged, keep: u32, first: u32, recent: u32, scratch: *const rcu_tensor) -> rcu_status;
+    pub fn rcu_paged_evict_scratch(dev: *mut rcu_device, cache: *const rcu_paged, keep: u32) -> u64;
     pub fn rcu_lazy_from_host(dev: *mut rcu_device, dt: i32, rank: u32, shape: *const u64, host: *const c_void, nbytes: u64, out: *mut *mut rcu_lazy) -> rcu_status;
     pub fn rcu_lazy_zeros(dev: *mut rcu_device, dt: i32, rank: u32, shape: *const u64, out: *mut *mut rcu_lazy) -> rcu_status;
     pub fn rcu_lazy_wrap(dev: *mut rcu_device, t: *const rcu_tensor, out: *mut *mut rcu_lazy) -> rcu_status;
@@ -326,6 +348,21 @@ extern "C" {
     ) -> rcu_status;
     pub fn rcu_lazy_window_attention(
         q: *mut rcu_lazy, kv: *mut rcu_lazy, shared: *mut rcu_lazy, shared_col: u32, vdim: u32, window: u32, scale: f32, out: *mut *mut rcu_lazy,
+    ) -> rcu_status;
+    pub fn rcu_lazy_rotary_axes(
+        x: *mut rcu_lazy, x_col: u32, heads: u32, dim: u32, first: u32, freqs: *mut rcu_lazy, magnitude: f32, positions: *mut rcu_lazy, sections: *const u32, halves: c_int, out: *mut *mut rcu_lazy,
+    ) -> rcu_status;
+    pub fn rcu_lazy_paged_append(
+        k: *mut rcu_lazy, k_col: u32, v: *mut rcu_lazy, v_col: u32, keys: *mut rcu_lazy, values: *mut rcu_lazy, table: *mut rcu_lazy, starts: *mut rcu_lazy, lengths: *mut rcu_lazy, mass: *mut rcu_lazy,
+        out: *mut *mut rcu_lazy,
+    ) -> rcu_status;
+    pub fn rcu_lazy_paged_attention(
+        q: *mut rcu_lazy, keys: *mut rcu_lazy, values: *mut rcu_lazy, table: *mut rcu_lazy, starts: *mut rcu_lazy, lengths: *mut rcu_lazy, mass: *mut rcu_lazy, sink: *mut rcu_lazy, window: u32, first: u32,
+        scale: f32, out: *mut *mut rcu_lazy,
+    ) -> rcu_status;
+    pub fn rcu_lazy_paged_evict(
+        keys: *mut rcu_lazy, values: *mut rcu_lazy, table: *mut rcu_lazy, lengths: *mut rcu_lazy, mass: *mut rcu_lazy, into_keys: *mut rcu_lazy, into_values: *mut rcu_lazy, into_table: *mut rcu_lazy,
+        into_mass: *mut rcu_lazy, keep: u32, first: u32, recent: u32, out: *mut *mut rcu_lazy,
     ) -> rcu_status;
     pub fn rcu_lazy_id(t: *const rcu_lazy) -> u64;
     pub fn rcu_lazy_execution_order(t: *mut rcu_lazy, ids: *mut u64, capacity: u32, n_nodes: *mut u32) -> rcu_status;

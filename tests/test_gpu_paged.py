@@ -1,0 +1,441 @@
+"""Operators over paged caches through the device ABI against the plain float64 restatement (paged_plain.py): rotation by given positions,
+append, attention and eviction, alone and in a run as a server makes it."""
+import numpy as np
+import pytest
+
+from ratchet_b200 import PagedCache, RatchetCudaError, Tensor, capi, nn
+
+from . import paged_plain as pp
+from .paged_plain import BF16, F16, F32, HALF_STEP
+from .test_gpu_dadezen_ops import dev, rng  # noqa: F401  (dev is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+DTS = [F32, F16, BF16]
+
+
+def up(dev, a, dt=None):
+    return dev.from_numpy(np.ascontiguousarray(a), dt=dt)
+
+
+def put(dev, a, dt):
+    h, v = pp.encode(a, dt)
+    return up(dev, h, dt), v
+
+
+def get(buf):
+    return pp.decode(buf.to_numpy(), buf.dt)
+
+
+def device_cache(dev, c, mass=None):
+    i = lambda a: up(dev, np.asarray(a, np.int32))  # noqa: E731
+    m = None if mass is None else up(dev, mass.astype(np.float32))
+    return PagedCache(up(dev, c.keys, c.dt), up(dev, c.values, c.dt), i(c.table), i(c.lengths), i(c.starts), m)
+
+
+def close(got, want, size, dt, vmax):
+    """Elementwise: the output's rounding, the rounding of every weight to the operands' type (16 bits: half a step of sum w |v|), and f32
+    arithmetic: scores of up to 256 products are off by about 16 half steps of their terms' size (some 10 for the inputs here: 1e-5), which
+    moves a weight by as much relative to itself, hence the sum by 2e-5 of the largest value."""
+    h = HALF_STEP[dt]
+    bound = h * (np.abs(want) + (size if dt != F32 else 0)) * 1.02 + 2e-5 * vmax
+    return float(np.max((np.abs(got - want) - bound) / vmax)) <= 0
+
+
+# ---------------------------------------------------------------------------------------- rotation
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("T,H,D,first,sections,col,halves", [
+    (1, 1, 8, 0, (4,), 0, False), (5, 3, 64, 0, (32,), 8, True), (33, 2, 80, 0, (8, 16, 16), 0, True), (7, 4, 128, 16, (10, 6, 20, 4), 16, False),
+    (300, 6, 96, 0, (48,), 0, False), (9, 3, 20, 3, (5,), 1, True), (9, 2, 14, 2, (2, 3), 3, False), (4, 1, 256, 64, (0, 32, 16), 0, True)])
+def test_rotary_axes(dev, dt, T, H, D, first, sections, col, halves):
+    g = rng(T * D + col)
+    pairs = sum(sections)
+    f = 10000.0 ** (-np.arange(pairs) / pairs)
+    hi = f.astype(np.float32)
+    freqs = up(dev, np.stack([hi, (f - hi).astype(np.float32)]))
+    # far positions, negative ones, and the ends of the type
+    at = g.integers(-200000, 2 ** 20, (len(sections), T)).astype(np.int32)
+    at[0, 0], at[-1, -1] = 2 ** 31 - 1, -2 ** 31
+    x, xv = put(dev, g.standard_normal((T, col + H * D + 8)), dt)
+    got = get(dev.rotary_axes(x, H, D, freqs, up(dev, at), sections, magnitude=1.25, col=col, first=first, halves=halves))
+    want = pp.rotary(xv[:, col:col + H * D].reshape(T, H, D), f, at, sections, 1.25, first, halves)
+    # the output's rounding; a cosine's (two half steps of f32 and its own), times two terms of size 1.25 * 5; the table: 2^-48 of an angle of 2^31
+    assert np.all(np.abs(got - want) <= HALF_STEP[dt] * np.abs(want) + 8 * 2.0 ** -24 * 1.25 * np.abs(xv).max() + 2.0 ** -16 * np.abs(xv).max())
+    assert np.array_equal(np.delete(got, np.arange(first, first + 2 * pairs), 2), np.delete(xv[:, col:col + H * D].reshape(T, H, D), np.arange(first, first + 2 * pairs), 2))
+
+
+def test_rotary_axes_near_positions_are_exact_to_f32(dev):
+    g = rng(3)
+    f = 500.0 ** (-np.arange(32) / 32)
+    hi = f.astype(np.float32)
+    at = np.concatenate([np.arange(50), [131071, 999983]]).astype(np.int32)[None]
+    x, xv = put(dev, g.standard_normal((52, 3 * 64)), F32)
+    want = pp.rotary(xv.reshape(52, 3, 64), f, at, (32,), 1.0, 0, False)
+    buf = x
+    got = get(dev.rotary_axes(buf, 3, 64, up(dev, np.stack([hi, (f - hi).astype(np.float32)])), up(dev, at), (32,), out=buf.view((52, 3, 64))))       # in place
+    assert np.abs(got - want).max() < 6 * 2.0 ** -24 * np.abs(xv).max()
+
+
+# ---------------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("new,lengths,G,D,E,R,k_col,v_col", [
+    ([1], [1], 1, 8, 8, 16, 0, 0), ([3, 0, 17, 1], [3, 9, 40, 33], 2, 24, 40, 16, 8, 16), ([40], [100], 6, 64, 64, 32, 0, 3), ([0, 0], [5, 0], 1, 16, 8, 16, 0, 0),
+    ([1] * 70, list(range(1, 71)), 2, 80, 80, 64, 1, 0), ([130, 2], [130, 1024], 3, 256, 128, 1024, 0, 0)])
+def test_append(dev, dt, new, lengths, G, D, E, R, k_col, v_col):
+    g = rng(sum(lengths) + D)
+    c = pp.Cache(g, dt, new, lengths, G, D, E, R, fill=0.5)
+    T = sum(new)
+    k, kv = put(dev, g.standard_normal((T + 3, k_col + G * D + 5)), dt)          # three rows belong to no sequence
+    v, vv = put(dev, g.standard_normal((T + 3, v_col + G * E)), dt)
+    mass = g.random((len(new), G, c.rows)) + 1
+    d = device_cache(dev, c, mass)
+    dev.paged_append(k, v, d, k_col=k_col, v_col=v_col)
+    keys, values, want_m = pp.decode(c.keys, dt), pp.decode(c.values, dt), mass.astype(np.float32)
+    for s, (n, L) in enumerate(zip(new, lengths)):
+        for i in range(n):
+            r, t = L - n + i, c.starts[s] + i
+            p = c.table[s, r // R]
+            keys[p, :, r % R] = kv[t, k_col:k_col + G * D].reshape(G, D)
+            values[p, :, r % R] = vv[t, v_col:v_col + G * E].reshape(G, E)
+            want_m[s, :, r] = 0
+    assert np.array_equal(get(d.keys), keys) and np.array_equal(get(d.values), values) and np.array_equal(d.mass.to_numpy(), want_m)
+    dev.sync()
+
+
+# ---------------------------------------------------------------------------------------- attention
+# new tokens, rows with them, H, G, D, E, page rows, window, first, sink
+SHAPES = [
+    ([1], [1], 1, 1, 8, 8, 16, 0, 0, False),
+    ([1, 1, 1], [5, 128, 129], 4, 2, 64, 64, 16, 0, 0, True),
+    ([3, 0, 1, 20], [3, 7, 300, 50], 6, 2, 96, 96, 32, 0, 0, False),
+    ([70, 1], [200, 513], 7, 1, 80, 80, 64, 0, 0, False),
+    ([129], [129], 4, 4, 128, 128, 128, 0, 0, False),
+    ([300], [700], 8, 2, 128, 64, 256, 100, 4, True),
+    ([1, 40], [1000, 1000], 10, 2, 64, 128, 16, 1, 0, False),
+    ([1, 9], [600, 300], 16, 1, 112, 48, 32, 130, 200, False),
+    ([17], [33], 3, 1, 24, 40, 16, 5, 1, True),
+    ([6, 1], [260, 90], 2, 2, 256, 256, 64, 0, 0, False),
+    ([33], [4100], 4, 2, 128, 128, 1024, 0, 0, False),
+    ([1] * 40, [3 * i + 1 for i in range(40)], 5, 5, 64, 64, 16, 20, 2, False),
+    ([2, 260], [2, 260], 130, 1, 16, 16, 16, 0, 0, False),
+]
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("new,lengths,H,G,D,E,R,window,first,sink", SHAPES)
+def test_attention(dev, dt, new, lengths, H, G, D, E, R, window, first, sink):
+    g = rng(sum(lengths) + H)
+    c = pp.Cache(g, dt, new, lengths, G, D, E, R)
+    T, scale = sum(new), 1.0 / np.sqrt(D)
+    q, qv = put(dev, 1.5 * g.standard_normal((T, H, D)), dt)
+    sk = g.standard_normal(H).astype(np.float32) if sink else None
+    want, size, mass = pp.attention(c, qv, scale, sk, window, first)
+    vmax = max(np.abs(v).max() for v in c.v if v.size)
+    skb = up(dev, sk) if sink else None
+    got = get(dev.paged_attention(q, device_cache(dev, c), scale, skb, window, first)).reshape(T, H, E)
+    assert close(got, want, size, dt, vmax)
+    # with the weights summed: the same outputs, and sums whose terms are off by what scores are off by (2e-5, see close)
+    before = g.random((len(new), G, c.rows)).astype(np.float32)
+    d = device_cache(dev, c, before)
+    again = get(dev.paged_attention(q, d, scale, skb, window, first)).reshape(T, H, E)
+    assert np.array_equal(again, got)
+    grown = d.mass.to_numpy().astype(np.float64) - before
+    for s, L in enumerate(lengths):
+        assert np.all(np.abs(grown[s, :, :L] - mass[s]) <= 2e-5 * mass[s] + 4 * 2.0 ** -24 * (1 + mass[s]))
+        assert np.all(grown[s, :, L:] == 0)
+    dev.sync()
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("H,G,D,n,L,window", [(4, 1, 64, 150, 290, 0), (2, 2, 128, 130, 130, 40), (8, 2, 80, 1, 300, 0), (3, 1, 24, 20, 40, 7)])
+def test_attention_of_values_that_are_not_finite(dev, dt, H, G, D, n, L, window):
+    """Infinities and NaN among the values and keys reach the tokens that see them, and no others."""
+    g = rng(L + H)
+    c = pp.Cache(g, dt, [n], [L], G, D, D, 16)
+    q, qv = put(dev, g.standard_normal((n, H, D)), dt)
+    places = [(L - 1, 0, np.inf), (L - max(1, n // 2), 1, -np.inf), (max(0, L - n - 3), 2, np.nan), (L // 3, 3, np.inf)]
+    keys, values = pp.decode(c.keys, dt), pp.decode(c.values, dt)
+    for r, d, x in places:
+        c.v[0][r, 0, d] = values[c.table[0, r // 16], 0, r % 16, d] = x
+    bad = L - 2 if n > 2 else None
+    if bad is not None:                                     # a key: NaN for who sees it
+        c.k[0][bad, 0, 0] = keys[c.table[0, bad // 16], 0, bad % 16, 0] = np.nan
+    c.keys, c.values = pp.encode(keys, dt)[0], pp.encode(values, dt)[0]
+    with np.errstate(invalid="ignore"):
+        want, size, _ = pp.attention(c, qv, 0.125, None, window)
+    got = get(dev.paged_attention(q, device_cache(dev, c), 0.125, window=window)).reshape(n, H, D)
+    fine = np.isfinite(want)
+    assert fine.any() and np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isposinf(got), np.isposinf(want))
+    assert close(np.where(fine, got, 0), np.where(fine, want, 0), np.where(np.isfinite(size), size, 0), dt, 5.0)
+
+
+@pytest.mark.parametrize("dt", DTS)
+def test_attention_leaves_rows_of_no_sequence(dev, dt):
+    g = rng(11)
+    c = pp.Cache(g, dt, [3, 5], [30, 5], 2, 64, 64, 16)
+    q, qv = put(dev, g.standard_normal((12, 4, 64)), dt)
+    c.starts = np.array([2, 5, 10], np.int32)               # two tokens before the first sequence, two behind the last
+    out = up(dev, pp.encode(np.full((12, 256), 7.0), dt)[0], dt)
+    dev.paged_attention(q, device_cache(dev, c), 0.125, out=out)
+    want, size, _ = pp.attention(c, qv, 0.125)
+    got = get(out)
+    assert np.all(got[[0, 1, 10, 11]] == 7)
+    assert close(got[2:10].reshape(8, 4, 64), want[2:10], size[2:10], dt, 5.0)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 40.0])
+@pytest.mark.parametrize("dt", DTS)
+def test_attention_scales(dev, dt, scale):
+    g = rng(5)
+    c = pp.Cache(g, dt, [60, 1], [200, 77], 1, 32, 32, 16)
+    q, qv = put(dev, g.standard_normal((61, 2, 32)), dt)
+    want, size, _ = pp.attention(c, qv, scale)
+    got = get(dev.paged_attention(q, device_cache(dev, c), scale)).reshape(61, 2, 32)
+    # scores of a few hundred: f32 keeps them to 2^-24 of their terms, some 40 * 32, which is 1e-4 of a weight
+    assert np.all(np.abs(got - want) <= HALF_STEP[dt] * (np.abs(want) + (size if dt != F32 else 0)) * 1.02 + 1e-3)
+
+
+def test_shared_pages_and_scratch_of_the_caller(dev):
+    """Two sequences over the same prompt's pages, twice on one scratch."""
+    g = rng(21)
+    c = pp.Cache(g, BF16, [1, 1], [64, 64], 2, 64, 64, 32)
+    c.table[1] = c.table[0]
+    c.k[1], c.v[1] = c.k[0], c.v[0]
+    q, qv = put(dev, g.standard_normal((2, 4, 64)), BF16)
+    d = device_cache(dev, c)
+    scratch = dev.empty(F32, (max(1, dev.paged_attention_scratch(q, d) // 4),))
+    want, size, _ = pp.attention(c, qv, 0.125)
+    for _ in range(2):
+        got = get(dev.paged_attention(q, d, 0.125, scratch=scratch)).reshape(2, 4, 64)
+        assert close(got, want, size, BF16, 5.0)
+
+
+# ---------------------------------------------------------------------------------------- eviction
+EVICT = [
+    ([100], 2, 24, 40, 16, 40, 4, 10), ([5, 33, 0, 300], 3, 64, 64, 32, 33, 0, 0), ([1000, 999], 1, 8, 8, 16, 1000, 1000, 0), ([700], 2, 128, 128, 64, 64, 0, 64),
+    ([3000, 17, 1500], 2, 96, 64, 256, 1025, 7, 300), ([40, 41], 6, 16, 16, 16, 1, 0, 0), ([5000], 1, 256, 256, 1024, 4999, 1, 1), ([64], 70, 8, 16, 16, 9, 1, 2)]
+
+
+def masses(g, S, G, rows):
+    """Many ties, zeros of both signs, infinities and NaN."""
+    m = np.round(g.exponential(3.0, (S, G, rows)), 0).astype(np.float32)
+    m[g.random(m.shape) < 0.1] *= -1.0
+    m[g.random(m.shape) < 0.02] = np.nan
+    m[g.random(m.shape) < 0.01] = np.inf
+    m[g.random(m.shape) < 0.01] = -np.inf
+    return m
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("place", ["fresh", "same", "pages"])
+@pytest.mark.parametrize("lengths,G,D,E,R,keep,first,recent", EVICT)
+def test_evict(dev, dt, place, lengths, G, D, E, R, keep, first, recent):
+    g = rng(sum(lengths) + keep)
+    S = len(lengths)
+    most = max(1, -(-min(keep, max(lengths)) // R))
+    c = pp.Cache(g, dt, [0] * S, lengths, G, D, E, R, spare=S * most + 3, fill=0.25)
+    mass = masses(g, S, G, c.rows)
+    d = device_cache(dev, c, mass)
+    new_lengths = up(dev, np.full(S, -5, np.int32))
+    if place == "fresh":                                    # other arrays
+        table = g.permutation(S * most + 1)[:S * most].reshape(S, most).astype(np.int32)
+        blank = lambda w: up(dev, pp.encode(np.full((S * most + 1, G, R, w), 0.75), dt)[0], dt)  # noqa: E731
+        into = PagedCache(blank(D), blank(E), up(dev, table), new_lengths, mass=up(dev, np.full((S, G, most * R), 9, np.float32)))
+    elif place == "pages":                                  # free pages of the same arrays
+        table = c.free[:S * most].reshape(S, most).astype(np.int32)
+        into = PagedCache(d.keys, d.values, up(dev, table), new_lengths, mass=up(dev, np.full((S, G, most * R), 9, np.float32)))
+    else:                                                   # in place
+        table = c.table
+        into = PagedCache(d.keys, d.values, d.table, new_lengths, mass=d.mass)
+    dev.paged_evict(d, into, keep, first, recent)
+    keys, values, sums = into.keys.to_numpy(), into.values.to_numpy(), into.mass.to_numpy()
+    assert np.array_equal(new_lengths.to_numpy(), np.minimum(lengths, keep))
+    for s, L in enumerate(lengths):
+        n = min(L, keep)
+        got_k, got_v = c.rows_of(keys, table, s, n), c.rows_of(values, table, s, n)
+        for h in range(G):
+            rows = pp.kept(mass[s, h], L, keep, first, recent)
+            assert np.array_equal(got_k[:, h], c.k[s][rows, h]) and np.array_equal(got_v[:, h], c.v[s][rows, h])
+            assert np.array_equal(sums[s, h, :n], mass[s, h, rows], equal_nan=True)
+            if place != "same":
+                assert np.all(sums[s, h, n:] == 9)
+    dev.sync()
+
+
+# ---------------------------------------------------------------------------------------- together
+def serve(dev, dt, step, evict):
+    """Three sequences: prompts, then single tokens, their rows cut to 40 whenever one has more than 60; against float64 all the way."""
+    g = rng(8)
+    H, G, D, R, MP, keep, first, recent = 4, 2, 64, 16, 8, 40, 2, 12
+    rows = MP * R
+    k64, v64, m64 = [[np.zeros((0, G, D)) for _ in range(3)] for _ in range(2)] + [[np.zeros((G, 0)) for _ in range(3)]]
+    for new in [[50, 20, 0], [1, 1, 33], [9, 1, 1], [1, 1, 1], [30, 0, 1], [1, 1, 60]]:
+        T = sum(new)
+        q, k, v = (pp.encode(g.standard_normal((T, n * D)), dt) for n in (H, G, G))
+        c = pp.Cache.__new__(pp.Cache)
+        c.dt, c.new, c.G, c.D, c.E, c.R = dt, new, G, D, D, R
+        c.starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        for s, n in enumerate(new):
+            t = c.starts[s]
+            k64[s] = np.concatenate([k64[s], k[1][t:t + n].reshape(n, G, D)])
+            v64[s] = np.concatenate([v64[s], v[1][t:t + n].reshape(n, G, D)])
+            m64[s] = np.concatenate([m64[s], np.zeros((G, n))], 1)
+        c.k, c.v, c.lengths = k64, v64, [len(x) for x in k64]
+        want, size, mass = pp.attention(c, q[1].reshape(T, H, D), 0.125)
+        got = step(q[0].reshape(T, H, D), k[0], v[0], c.starts, np.asarray(c.lengths, np.int32))
+        assert close(pp.decode(got, dt).reshape(T, H, D), want, size, dt, 5.0)
+        m64 = [a + b for a, b in zip(m64, mass)]
+        if max(c.lengths) > 60:
+            m, lengths = evict(keep, first, recent)
+            assert np.array_equal(lengths, np.minimum(c.lengths, keep))
+            for s, L in enumerate(c.lengths):
+                k2, v2, m2 = [], [], []
+                for h in range(G):
+                    at = pp.kept(m64[s][h], L, keep, first, recent)
+                    assert np.allclose(m[s, h, :len(at)], m64[s][h][at], rtol=1e-4, atol=1e-6)
+                    k2.append(k64[s][at, h])
+                    v2.append(v64[s][at, h])
+                    m2.append(m64[s][h][at])
+                k64[s], v64[s], m64[s] = np.stack(k2, 1), np.stack(v2, 1), np.stack(m2)
+    return rows
+
+
+@pytest.mark.parametrize("dt", DTS)
+def test_a_run_of_calls(dev, dt):
+    G, D, R, MP = 2, 64, 16, 8
+    table = up(dev, rng(1).permutation(3 * MP).reshape(3, MP).astype(np.int32))
+    keys, values = dev.zeros(dt, (3 * MP, G, R, D)), dev.zeros(dt, (3 * MP, G, R, D))
+    mass, cut = dev.zeros(F32, (3, G, MP * R)), dev.zeros(capi.I32, (3,))
+    last = {}
+
+    def step(q, k, v, starts, lengths):
+        last["c"] = c = PagedCache(keys, values, table, up(dev, lengths), up(dev, starts), mass)
+        dev.paged_append(up(dev, k, dt), up(dev, v, dt), c)
+        return dev.paged_attention(up(dev, q, dt), c, 0.125).to_numpy()
+
+    def evict(keep, first, recent):
+        dev.paged_evict(last["c"], PagedCache(keys, values, table, cut, mass=mass), keep, first, recent)
+        return mass.to_numpy(), cut.to_numpy()
+
+    serve(dev, dt, step, evict)
+
+
+@pytest.mark.parametrize("dt", [F16, F32])
+def test_a_run_of_the_graph(dev, dt):
+    """The same through the lazy graph: rows that the graph computes, nodes ordered by the lengths they hand on."""
+    G, D, R, MP = 2, 64, 16, 8
+    leaf = lambda a: Tensor.from_data(a, device=dev)  # noqa: E731
+    host = np.float16 if dt == F16 else np.float32
+    table = leaf(rng(1).permutation(3 * MP).reshape(3, MP).astype(np.int32))
+    keys, values = leaf(np.zeros((3 * MP, G, R, D), host)), leaf(np.zeros((3 * MP, G, R, D), host))
+    mass = leaf(np.zeros((3, G, MP * R), np.float32))
+    last = {}
+
+    def step(q, k, v, starts, lengths):
+        c = nn.PagedState(keys, values, table, leaf(starts), leaf(lengths), mass)
+        # keys and values through a node of the graph: a sum with zeros
+        after = leaf(k).add(leaf(np.zeros_like(k))).paged_append(leaf(v), c)
+        last["c"] = after
+        return leaf(q).paged_attention(after, 0.125).to_numpy()
+
+    def evict(keep, first, recent):
+        lengths = last["c"].evict(nn.PagedState(keys, values, table, None, None, mass), keep, first, recent).lengths.to_numpy()
+        return mass.to_numpy(), lengths
+
+    serve(dev, dt, step, evict)
+
+
+# ---------------------------------------------------------------------------------------- refusals
+def test_bad_indexes_are_reported(dev):
+    g = rng(2)
+
+    def reported(change, call):
+        c = pp.Cache(g, F16, [2, 1], [20, 5], 1, 64, 64, 16, fill=0.0)
+        change(c)
+        call(device_cache(dev, c, np.zeros((2, 1, c.rows))))
+        with pytest.raises(RatchetCudaError) as e:
+            dev.sync()
+        assert e.value.status == capi.ERR_BOUNDS
+        dev.sync()                                          # reported once
+
+    q, _ = put(dev, g.standard_normal((3, 2, 64)), F16)
+    k, _ = put(dev, g.standard_normal((3, 64)), F16)
+    attend = lambda d: dev.paged_attention(q, d, 0.1)  # noqa: E731
+    append = lambda d: dev.paged_append(k, k, d)  # noqa: E731
+
+    def setter(name, at, value):
+        def change(c):
+            a = np.array(getattr(c, name))
+            a[at] = value
+            setattr(c, name, a)
+        return change
+
+    for call in (attend, append):
+        for change in (setter("starts", 1, 4), setter("starts", 2, -1), setter("starts", 0, 3), setter("lengths", 0, 33), setter("lengths", 1, -1),
+                       setter("lengths", 0, 1), setter("table", (0, 1), 99), setter("table", (1, 0), -7)):
+            reported(change, call)
+    for change in (setter("lengths", 0, 40), setter("table", (0, 1), 1000)):
+        def evict(d):
+            into = PagedCache(dev.zeros(F16, (4, 1, 16, 64)), dev.zeros(F16, (4, 1, 16, 64)), up(dev, np.array([[0], [1]], np.int32)), dev.zeros(capi.I32, (2,)),
+                              mass=dev.zeros(F32, (2, 1, 16)))
+            dev.paged_evict(d, into, 10, 2, 8)
+        reported(change, evict)
+
+
+def test_refusals(dev):
+    z = lambda dt, *shape: dev.zeros(dt, shape)  # noqa: E731
+    I32 = capi.I32
+
+    def cache(dt=F16, pages=4, G=2, R=16, D=64, E=64, S=2, MP=2, mass=False, **other):
+        parts = {"keys": z(dt, pages, G, R, D), "values": z(dt, pages, G, R, E), "table": z(I32, S, MP), "lengths": z(I32, S), "starts": z(I32, S + 1),
+                 "mass": z(F32, S, G, MP * R) if mass else None}
+        parts.update(other)
+        return PagedCache(**parts)
+
+    q, k, x = z(F16, 3, 4, 64), z(F16, 3, 128), z(F16, 3, 256)
+    fr, at = z(F32, 2, 32), z(I32, 1, 3)
+    dev.paged_attention(q, cache(), 0.1)
+    dev.paged_append(k, k, cache())
+    dev.rotary_axes(x, 4, 64, fr, at, (32,))
+    dev.paged_evict(cache(mass=True), cache(mass=True), 8)
+    dev.sync()
+    bad = [
+        lambda: dev.paged_attention(z(F32, 3, 4, 64), cache(), 0.1), lambda: dev.paged_attention(z(F16, 3, 4, 32), cache(), 0.1),
+        lambda: dev.paged_attention(z(F16, 3, 3, 64), cache(), 0.1), lambda: dev.paged_attention(q, cache(), 0.1, sink=z(F32, 2)),
+        lambda: dev.paged_attention(q, cache(), 0.1, out=z(F16, 3, 128)), lambda: dev.paged_attention(q, cache(R=8), 0.1), lambda: dev.paged_attention(q, cache(R=24), 0.1),
+        lambda: dev.paged_attention(z(F16, 3, 4, 60), cache(D=60), 0.1), lambda: dev.paged_attention(z(F16, 3, 4, 264), cache(D=264), 0.1),
+        lambda: dev.paged_attention(q, cache(starts=z(I32, 2)), 0.1), lambda: dev.paged_attention(q, cache(lengths=z(I32, 3)), 0.1),
+        lambda: dev.paged_attention(q, cache(lengths=z(F32, 2)), 0.1), lambda: dev.paged_attention(q, cache(starts=None), 0.1),
+        lambda: dev.paged_attention(q, cache(mass=True, table=z(I32, 2, 3)), 0.1), lambda: dev.paged_attention(q, cache(values=z(F16, 5, 2, 16, 64)), 0.1),
+        lambda: dev.paged_attention(q, cache(values=z(BF16, 4, 2, 16, 64)), 0.1),
+        lambda: dev.paged_append(k, z(F16, 2, 128), cache()), lambda: dev.paged_append(k, k, cache(), k_col=1), lambda: dev.paged_append(z(F32, 3, 128), k, cache()),
+        lambda: dev.paged_evict(cache(), cache(mass=True), 8), lambda: dev.paged_evict(cache(mass=True), cache(), 8), lambda: dev.paged_evict(cache(mass=True), cache(mass=True), 0),
+        lambda: dev.paged_evict(cache(mass=True), cache(mass=True), 8, 5, 4), lambda: dev.paged_evict(cache(mass=True), cache(mass=True, MP=1), 17),
+        lambda: dev.paged_evict(cache(mass=True), cache(mass=True, S=3), 8), lambda: dev.paged_evict(cache(mass=True), cache(mass=True, dt=BF16), 8),
+        lambda: dev.rotary_axes(x, 4, 64, fr, at, (31,)), lambda: dev.rotary_axes(x, 4, 64, fr, at, (16, 16)), lambda: dev.rotary_axes(x, 4, 64, fr, at, (32,), col=1),
+        lambda: dev.rotary_axes(x, 4, 64, fr, at, (32,), first=1), lambda: dev.rotary_axes(x, 4, 64, fr, z(I32, 1, 2), (32,)),
+        lambda: dev.rotary_axes(x, 4, 64, fr, z(I32, 5, 3), (32, 0, 0, 0, 0)), lambda: dev.rotary_axes(x, 4, 64, fr, z(F32, 1, 3), (32,)),
+        lambda: dev.rotary_axes(x, 2, 64, fr, at, (32,), out=dev.wrap(F16, (3, 2, 64), x.ptr)),
+    ]
+    m = cache(mass=True)
+    bad += [lambda: dev.paged_evict(m, m, 8), lambda: dev.paged_evict(m, PagedCache(m.keys, m.values, m.table, m.lengths, mass=m.mass), 8),
+            lambda: dev.paged_evict(m, PagedCache(m.values, m.keys, m.table, z(I32, 2), mass=m.mass), 8)]
+    for f in bad:
+        with pytest.raises(RatchetCudaError):
+            f()
+    dev.sync()
+
+
+def test_scratch_that_is_too_small_is_refused(dev):
+    g = rng(4)
+    c = pp.Cache(g, F16, [1], [3000], 2, 64, 64, 16)
+    q, _ = put(dev, g.standard_normal((1, 4, 64)), F16)
+    d = device_cache(dev, c, np.zeros((1, 2, c.rows)))
+    assert dev.paged_attention_scratch(q, d) > 16
+    with pytest.raises(RatchetCudaError):
+        dev.paged_attention(q, d, 0.1, scratch=dev.zeros(F32, (4,)))
+    into = PagedCache(d.keys, d.values, d.table, dev.zeros(capi.I32, (1,)), mass=d.mass)
+    with pytest.raises(RatchetCudaError):
+        dev.paged_evict(d, into, 100, scratch=dev.zeros(F32, (4,)))
+    dev.paged_evict(d, into, 100, scratch=dev.zeros(F32, (dev.paged_evict_scratch(d, 100) // 4,)))
+    dev.sync()
