@@ -4,49 +4,11 @@
 //
 // over the rows j that the token at row r sees: j <= r, and with a window j > r - window or j < first.
 #include "paged_attention.cuh"
+#include "paged_rows.cuh"
 
 namespace {
 
 using namespace paged;
-
-// rows that the token at row r sees: [0, head) and [low, r + 1)
-__device__ __forceinline__ void visible(const AttendArgs& a, int r, int& head, int& low) {
-    low = a.window > 0 && r >= a.window ? r - a.window + 1 : 0;
-    head = min(a.first, low);
-}
-
-// A warp's pass over rows [j0, j1) of a sequence for one query: 32 keys a step, a lane for each; then a lane for every 32nd feature of the values.
-template <class T>
-__device__ void attend_run(const AttendArgs& a, int s, int g, const T* q, int j0, int j1, float& m, float& l, float (&o)[8]) {
-    const View& p = a.p;
-    const int lane = threadIdx.x & 31;
-    const T *keys = (const T*)p.keys, *values = (const T*)p.values;
-    for (int j = j0; j < j1; j += 32) {
-        const int r = j + lane;
-        float z = -INFINITY;
-        int page = 0;
-        if (r < j1) {
-            page = page_of(p, s, r);
-            const T* k = keys + row_at(p, page, g, r, p.D);
-            float sum = 0.f;
-            for (int d = 0; d < p.D; ++d) sum = fmaf(to_f32<T>(q[d]), to_f32<T>(k[d]), sum);
-            z = sum * a.c;
-        }
-        const float next = fmaxf(m, warp_max(z)), base = next == -INFINITY ? 0.f : next;
-        const float corr = exp2f(m - base), w = r < j1 ? exp2f(z - base) : 0.f;
-        l = l * corr + warp_sum(w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] *= corr;
-        m = next;
-        for (int u = 0; u < min(32, j1 - j); ++u) {
-            const float pw = __shfl_sync(0xffffffffu, w, u);
-            const T* v = values + row_at(p, __shfl_sync(0xffffffffu, page, u), g, j + u, p.E);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (lane + 32 * i < p.E) o[i] = fmaf(pw, to_f32<T>(v[lane + 32 * i]), o[i]);
-        }
-    }
-}
 
 // A warp per token and head.
 template <class T>
@@ -62,28 +24,11 @@ __global__ void __launch_bounds__(128) attend_kernel(const AttendArgs a) {
     const int s = seq_of_token(p, t);
     if (s < 0) return;
     const Seq sq = seq_of(p, s);
-    const int r = min(sq.old() + t - sq.start, sq.L - 1), g = h / (a.H / p.G);
-    const T* q = (const T*)a.q + ((size_t)t * a.H + h) * p.D;
-    float m = -INFINITY, l = 0.f, o[8] = {};
-    int head, low;
-    visible(a, r, head, low);
-    if (r >= 0) {
-        attend_run<T>(a, s, g, q, 0, head, m, l, o);
-        attend_run<T>(a, s, g, q, low, r + 1, m, l, o);
-    }
-    if (a.sink && r >= 0) {
-        const float sk = a.sink[h] * kLog2e, next = fmaxf(m, sk), corr = exp2f(m - next);
-        l = l * corr + exp2f(sk - next);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] *= corr;
-        m = next;
-    }
-    const float inv = r >= 0 ? 1.f / l : 0.f;
-    T* out = (T*)a.out + ((size_t)t * a.H + h) * p.E;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < p.E) out[lane + 32 * i] = from_f32<T>(o[i] * inv);
-    if (a.lse && lane == 0) a.lse[(size_t)t * a.H + h] = r >= 0 ? m + log2f(l) : INFINITY;
+    const int r = min(sq.old() + t - sq.start, sq.L - 1);
+    RowPart part;
+    const Span sp = span_of(a.window, a.first, r, r);
+    attend_row<T>(a, s, h / (a.H / p.G), t, h, r, sp, 0, sp.count, part);
+    finish_row<T>(a, t, h, part);
 }
 
 // A warp per 32 rows of a sequence and kv head, a lane for each row: the weights that its tokens and heads give, in their order.
@@ -101,7 +46,7 @@ __global__ void __launch_bounds__(128) mass_kernel(const AttendArgs a) {
     for (int i = 0; i < sq.n; ++i) {
         const int r = sq.old() + i;
         int head, low;
-        visible(a, r, head, low);
+        visible(a.window, a.first, r, head, low);
         if (j > r || (j >= head && j < low)) continue;
         for (int h = g * per; h < (g + 1) * per; ++h) {
             const size_t at = (size_t)(sq.start + i) * a.H + h;
@@ -114,11 +59,16 @@ __global__ void __launch_bounds__(128) mass_kernel(const AttendArgs a) {
     p.mass[((size_t)s * p.G + g) * rows + j] += sum;
 }
 
-template <class T> rcu_status attend(rcu_device* dev, const AttendArgs& a) {
+template <class T> rcu_status attend(rcu_device* dev, const AttendArgs& a, int dt, bool tc, void* scratch) {
     const View& p = a.p;
-    const long long items = (long long)p.T * a.H;
-    rcu_launch(dev, attend_kernel<T>, (unsigned)((items + 3) / 4), 128, 0, a);
-    RCU_LAUNCH_CHECK(dev);
+    if (tc) {
+        const rcu_status st = attend_tc(dev, a, dt, scratch);
+        if (st != RCU_OK) return st;
+    } else {
+        const long long items = (long long)p.T * a.H;
+        rcu_launch(dev, attend_kernel<T>, (unsigned)((items + 3) / 4), 128, 0, a);
+        RCU_LAUNCH_CHECK(dev);
+    }
     if (p.mass) {
         rcu_launch(dev, mass_kernel<T>, dim3((unsigned)(((p.MP << p.shift) + 127) / 128), p.S * p.G), 128, 0, a);
         RCU_LAUNCH_CHECK(dev);
@@ -126,7 +76,12 @@ template <class T> rcu_status attend(rcu_device* dev, const AttendArgs& a) {
     return RCU_OK;
 }
 
-uint64_t scratch_bytes(const View& p, uint64_t H) { return p.mass ? align256((uint64_t)p.T * H * 4) : 0; }
+// lse of every query where mass is kept, and behind it what the tensor-core path takes (whether a call goes there is decided by more than the sizes)
+uint64_t lse_bytes(const View& p, uint64_t H) { return p.mass ? align256((uint64_t)p.T * H * 4) : 0; }
+uint64_t scratch_bytes(const rcu_device* dev, const View& p, uint64_t H, int dt) {
+    const bool tc = dt != RCU_F32 && p.D <= 128 && p.E <= 128 && H / p.G <= 128;
+    return lse_bytes(p, H) + (tc ? attend_tc_scratch(dev, p, (int)H) : 0);
+}
 
 }  // namespace
 
@@ -135,7 +90,8 @@ extern "C" {
 uint64_t rcu_paged_attention_scratch(rcu_device* dev, const rcu_tensor* q, const rcu_paged* cache) {
     View p;
     if (!dev || !t_valid(q) || q->rank != 3 || view(dev, "paged_attention", cache, q->shape[0], true, &p) != RCU_OK) return 0;
-    return scratch_bytes(p, q->shape[1]);
+    const uint64_t H = q->shape[1];
+    return H >= (uint64_t)p.G && H % p.G == 0 && H <= 65535 ? scratch_bytes(dev, p, H, q->dt) : 0;
 }
 
 rcu_status rcu_paged_attention(rcu_device* dev, const rcu_tensor* q, const rcu_paged* cache, const rcu_tensor* sink, uint32_t window, uint32_t first,
@@ -162,10 +118,12 @@ rcu_status rcu_paged_attention(rcu_device* dev, const rcu_tensor* q, const rcu_p
     a.c = scale * kLog2e;
     DevGuard guard(dev->ordinal);
     Scratch mem(dev);
-    st = mem.take("paged_attention", scratch, scratch_bytes(p, H));
+    st = mem.take("paged_attention", scratch, scratch_bytes(dev, p, H, q->dt));
     if (st != RCU_OK) return st;
     a.lse = p.mass ? (float*)mem.ptr : nullptr;
-    return q->dt == RCU_F32 ? attend<float>(dev, a) : q->dt == RCU_F16 ? attend<__half>(dev, a) : attend<__nv_bfloat16>(dev, a);
+    void* rest = (char*)mem.ptr + lse_bytes(p, H);
+    const bool tc = attend_tc_takes(dev, a, q->dt);
+    return q->dt == RCU_F32 ? attend<float>(dev, a, q->dt, tc, rest) : q->dt == RCU_F16 ? attend<__half>(dev, a, q->dt, tc, rest) : attend<__nv_bfloat16>(dev, a, q->dt, tc, rest);
 }
 
 }  // extern "C"

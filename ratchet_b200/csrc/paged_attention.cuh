@@ -1,4 +1,5 @@
-// What the kernels of attention over paged caches share (paged_attention.cu, paged_attention_tc.cu).
+// What the kernels of attention over paged caches share (paged_attention.cu, paged_attention_tc.cu): arguments, which rows a token sees, how
+// the work is cut, and the form of partial results.
 #pragma once
 #include "paged.cuh"
 
@@ -15,5 +16,110 @@ struct AttendArgs {
     int H, window, first;
     float c;                   // scale log2 e
 };
+
+#ifdef __CUDACC__
+// rows that the token at row r sees: [0, head) and [low, r + 1)
+__device__ __forceinline__ void visible(int window, int first, int r, int& head, int& low) {
+    low = window > 0 && r >= window ? r - window + 1 : 0;
+    head = min(first, low);
+}
+#endif
+
+// ------------------------------------------------------------------------------------------------ how the work is cut
+// An item is up to `tokens` consecutive new tokens of one sequence, with all heads of a group, over the tiles of kTileK rows that any of them
+// sees; an item exists once per kv head.  All items' tiles in a row, kv head by kv head, are cut into equal runs, one per CTA: a CTA takes
+// the end of one item, some whole ones and the beginning of another, whatever the lengths are.  Items that one CTA covers are finished by it,
+// the others' parts are joined by merge_kernel.  plan_kernel works this out on the device, where the lengths are.
+constexpr int kTileK = 128;
+
+struct Item {
+    int s, token, count, row;  // sequence; first token of the call, how many; row of the first one (s < 0: nothing to do)
+};
+struct Plan {
+    int items;                 // upper bound: T / tokens + S
+    int tokens;                // of an item
+    int ctas, least;           // CTAs at most; tiles that a CTA takes at least
+    int rows, stride;          // rows of a tile (tokens / 2 * group), of a part in scratch
+    // scratch
+    int* head;                 // [0] tiles of a kv head, [1] CTAs at work
+    int* prefix;               // [items + 1]: tiles of a kv head's items before each
+    Item* item;                // [items]
+    float2* ml;                // [2 * ctas, stride]: a part's maximum and sum, per row
+    float4* o;                 // [2 * ctas, E / 4, stride]: its weighted sum of values
+};
+
+#ifdef __CUDACC__
+// Tiles that tokens at rows r0 .. r1 see: the first `head` ones, then lo, lo + 1, ..
+struct Span {
+    int head, lo, count;
+    __device__ __forceinline__ int tile(int n) const { return n < head ? n : lo + n - head; }
+};
+__device__ __forceinline__ Span span_of(int window, int first, int r0, int r1) {
+    Span sp;
+    const int hi = r1 / kTileK + 1, low0 = window > 0 ? max(0, r0 - window + 1) : 0, low1 = window > 0 ? max(0, r1 - window + 1) : 0;
+    sp.lo = low0 / kTileK;
+    sp.head = (min(first, low1) + kTileK - 1) / kTileK;
+    if (sp.head >= sp.lo) sp.head = sp.lo = 0;
+    sp.count = r1 < 0 ? 0 : sp.head + hi - sp.lo;
+    return sp;
+}
+
+// The tiles that CTA b of C takes of `total`
+__device__ __forceinline__ int first_tile(long long total, int b, int C) { return (int)(total * b / C); }
+
+// A CTA's walk over its run: item by item
+struct Walk {
+    const Plan& pl;
+    int W, at, end, begin;     // tiles of a kv head; run
+    int g, i;                  // kv head and item at `at`
+    Item it;
+    int n0, n1, whole;         // tiles [n0, n1) of the item; whether these are all of them
+    __device__ __forceinline__ Walk(const Plan& plan, int b, int G) : pl(plan) {
+        W = plan.head[0];
+        const int C = plan.head[1];
+        const long long total = (long long)W * G;
+        at = begin = b < C ? first_tile(total, b, C) : 0;
+        end = b < C ? first_tile(total, b + 1, C) : 0;
+        if (at < end) find();
+    }
+    __device__ __forceinline__ void find() {
+        g = at / W;
+        const int y = at - g * W;
+        int lo = 0, hi = pl.items - 1;                  // the last item with prefix <= y
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (pl.prefix[mid] <= y) lo = mid;
+            else hi = mid - 1;
+        }
+        i = lo;
+        load();
+    }
+    __device__ __forceinline__ void load() {
+        it = pl.item[i];
+        const int p0 = g * W + pl.prefix[i], p1 = g * W + pl.prefix[i + 1];
+        n0 = at - p0;
+        n1 = min(end, p1) - p0;
+        whole = n0 == 0 && p0 + n1 == p1;
+    }
+    __device__ __forceinline__ bool more() const { return at < end; }
+    __device__ __forceinline__ int slot(int b) const { return 2 * b + (at != begin); }
+    __device__ __forceinline__ void next() {
+        at += n1 - n0;
+        if (at >= end) return;
+        if (at >= (g + 1) * W) {
+            ++g;
+            i = -1;
+        }
+        do ++i;
+        while (pl.prefix[i + 1] == pl.prefix[i]);       // ends: at < end <= W G, so a later item has tiles
+        load();
+    }
+};
+#endif
+
+// Any type, width and alignment (paged_attention.cu); f16 and bf16 up to 128 features on the tensor cores (paged_attention_tc.cu)
+bool attend_tc_takes(const rcu_device* dev, const AttendArgs& a, int dt);
+uint64_t attend_tc_scratch(const rcu_device* dev, const View& p, int H);
+rcu_status attend_tc(rcu_device* dev, const AttendArgs& a, int dt, void* scratch);
 
 }  // namespace paged
