@@ -62,13 +62,13 @@ __global__ void __launch_bounds__(128) mass_kernel(const AttendArgs a) {
 template <class T> rcu_status attend(rcu_device* dev, const AttendArgs& a, int dt, bool tc, void* scratch) {
     const View& p = a.p;
     if (tc) {
+        // the two run one after the other: they share the scratch
         const rcu_status st = attend_tc(dev, a, dt, scratch);
-        if (st != RCU_OK) return st;
-    } else {
-        const long long items = (long long)p.T * a.H;
-        rcu_launch(dev, attend_kernel<T>, (unsigned)((items + 3) / 4), 128, 0, a);
-        RCU_LAUNCH_CHECK(dev);
+        return st != RCU_OK || !p.mass ? st : mass_tc(dev, a, dt, scratch);
     }
+    const long long items = (long long)p.T * a.H;
+    rcu_launch(dev, attend_kernel<T>, (unsigned)((items + 3) / 4), 128, 0, a);
+    RCU_LAUNCH_CHECK(dev);
     if (p.mass) {
         rcu_launch(dev, mass_kernel<T>, dim3((unsigned)(((p.MP << p.shift) + 127) / 128), p.S * p.G), 128, 0, a);
         RCU_LAUNCH_CHECK(dev);
@@ -80,7 +80,8 @@ template <class T> rcu_status attend(rcu_device* dev, const AttendArgs& a, int d
 uint64_t lse_bytes(const View& p, uint64_t H) { return p.mass ? align256((uint64_t)p.T * H * 4) : 0; }
 uint64_t scratch_bytes(const rcu_device* dev, const View& p, uint64_t H, int dt) {
     const bool tc = dt != RCU_F32 && p.D <= 128 && p.E <= 128 && H / p.G <= 128;
-    return lse_bytes(p, H) + (tc ? attend_tc_scratch(dev, p, (int)H) : 0);
+    const uint64_t attend = tc ? attend_tc_scratch(dev, p, (int)H) : 0, mass = tc && p.mass ? mass_tc_scratch(dev, p, (int)H) : 0;
+    return lse_bytes(p, H) + (attend > mass ? attend : mass);
 }
 
 }  // namespace

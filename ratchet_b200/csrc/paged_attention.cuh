@@ -121,5 +121,8 @@ struct Walk {
 bool attend_tc_takes(const rcu_device* dev, const AttendArgs& a, int dt);
 uint64_t attend_tc_scratch(const rcu_device* dev, const View& p, int H);
 rcu_status attend_tc(rcu_device* dev, const AttendArgs& a, int dt, void* scratch);
+// the weights that every row receives, added to its mass; after the attention, whose lse it reads (paged_mass_tc.cu)
+uint64_t mass_tc_scratch(const rcu_device* dev, const View& p, int H);
+rcu_status mass_tc(rcu_device* dev, const AttendArgs& a, int dt, void* scratch);
 
 }  // namespace paged

@@ -18,26 +18,13 @@
 
 #include "paged_attention.cuh"
 #include "paged_rows.cuh"
-#include "tc_common.cuh"
+#include "paged_tc.cuh"
 
 namespace paged {
 namespace {
 
-using namespace tc;
+constexpr int kThreadsP = 320, kMostStages = 8;
 
-constexpr int kTileQ = 128, kThreadsP = 320, kBlock = 128 * 128;       // bytes of 64 columns of a tile of 128 rows
-constexpr int kMostStages = 8;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int u, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
-                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_u32(bar))
-                 : "memory");
-}
 template <class T> __device__ __forceinline__ uint32_t pack2(float x, float y);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
     const __half2 v = __floats2half2_rn(x, y);
@@ -487,17 +474,6 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a, const Pl
     }
 }
 
-bool map_4d(CUtensorMap* map, int dt, const void* base, const uint64_t (&dims)[4], uint32_t box1, uint32_t box3) {
-    gemvq8::EncodeTiledFn fn = gemvq8::encode_tiled_fn();
-    if (!fn) return false;
-    cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
-    cuuint64_t strides[3] = {dims[0] * 2, dims[0] * dims[1] * 2, dims[0] * dims[1] * dims[2] * 2};
-    cuuint32_t box[4] = {64, box1, 1, box3};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
-    return fn(map, dt == RCU_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), d, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // The cut of a call, and its scratch behind `mem` (nullable: sizes only); returns the bytes
 uint64_t plan_of(const rcu_device* dev, const View& p, int H, char* mem, Plan* out) {
     const int group = H / p.G, tq = kTileQ / group;
@@ -532,10 +508,7 @@ template <class T> rcu_status launch(rcu_device* dev, const AttendArgs& a, int d
     x.stages = room / x.stage_bytes < kMostStages ? room / x.stage_bytes : kMostStages;
     const size_t smem = 1024 + (size_t)2 * x.nb * kBlock + (size_t)x.stages * x.stage_bytes;
     CUtensorMap qm, km, vm;
-    const uint64_t qd[4] = {(uint64_t)p.D, (uint64_t)x.group, (uint64_t)p.G, (uint64_t)p.T}, kd[4] = {(uint64_t)p.D, (uint64_t)p.R, (uint64_t)p.G, (uint64_t)p.pages},
-                   vd[4] = {(uint64_t)p.E, (uint64_t)p.R, (uint64_t)p.G, (uint64_t)p.pages};
-    const uint32_t box = p.R < kTileK ? p.R : kTileK;
-    if (!map_4d(&qm, dt, a.q, qd, x.group, x.tq) || !map_4d(&km, dt, p.keys, kd, box, 1) || !map_4d(&vm, dt, p.values, vd, box, 1))
+    if (!map_queries(&qm, dt, p, a.q, x.group, x.tq) || !map_pages(&km, dt, p, p.keys, p.D) || !map_pages(&vm, dt, p, p.values, p.E))
         return rcu_fail(dev, RCU_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (%d tokens, %d heads, %d pages)", p.T, a.H, p.pages);
     rcu_launch(dev, plan_kernel, 1, 1024, 0, p, x.pl, a.window, a.first);
     RCU_LAUNCH_CHECK(dev);
@@ -558,7 +531,7 @@ bool attend_tc_takes(const rcu_device* dev, const AttendArgs& a, int dt) {
     const View& p = a.p;
     if (dt == RCU_F32 || p.D > 128 || p.E > 128 || a.H / p.G > kTileQ || !(a.c > 0.f) || !(a.c < INFINITY)) return false;
     // 32-bit tile numbers: all kv heads' tiles over the longest rows that the table allows
-    if ((uint64_t)(p.T / (2 * (kTileQ / (a.H / p.G))) + p.S) * (((uint64_t)p.MP << p.shift) / kTileK + 1) * p.G >= (1ull << 31)) return false;
+    if ((uint64_t)(p.T / (kTileQ / (a.H / p.G)) + p.S) * (((uint64_t)p.MP << p.shift) / kTileK + 1) * p.G >= (1ull << 31)) return false;
     return ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 && dev->smem_optin >= 227 * 1024;
 }
 

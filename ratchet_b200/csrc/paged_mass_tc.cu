@@ -1,0 +1,392 @@
+// The attention weight that every cached row receives (rcu_paged_attention where mass is kept), f16 and bf16 up to 128 features:
+//
+//   mass[j] += sum over the group's heads and the new tokens that see j of 2^(c q.k_j - lse(q))
+//
+// with the lse that the attention has left.  The scores are worked out again, the other way round: S^T = K Q^T has a row of the cache per lane of tensor
+// memory, so a thread adds up its own row's weights in a register, in the same order in every call, and nothing is exchanged between
+// lanes.  A tile of 128 rows stays in shared memory while the query tiles that see it pass by (paged_attention.cuh's cut, with rows and
+// queries in each other's place).
+//   warp 0            a tile of rows per item, two of them in turns; query tiles and their lse into a ring;
+//   warp 1            S^T of every query tile, four buffers of tensor memory;
+//   warps 2-5, 6-9    every other query tile each: exponentials and sums, which are joined at the end of the item.
+// Bound by the exponentials: 128 x 128 of them take 1024 cycles of an SM, the product half of that.
+// Every wait is bounded; one that gives up raises RCU_DEVFLAG_TIMEOUT and ends all others of the CTA.
+#include "paged_tc.cuh"
+
+namespace paged {
+namespace {
+
+constexpr int kThreadsM = 320, kStagesQ = 4;
+
+// Query tiles j of sequence q (tq tokens each) that see any of the rows j0 .. j0 + 127: [lo, hi)
+__device__ __forceinline__ void seen_by(const Seq& q, int window, int first, int tq, int j0, int& lo, int& hi) {
+    const int tiles = (q.n + tq - 1) / tq;
+    lo = j0 > q.old() ? (j0 - q.old()) / tq : 0;
+    hi = tiles;
+    if (window > 0 && j0 >= first) {
+        const int last = j0 + kTileK - 1 + window - 1 - q.old();         // the last token whose window reaches the tile
+        hi = last < 0 ? 0 : min(tiles, last / tq + 1);
+    }
+    lo = min(lo, hi);
+}
+
+// Items are tiles of rows: Item{sequence, tile, its first query tile, -}.  First the sequences' tiles before each (base), then as plan_kernel.
+__global__ void __launch_bounds__(1024) mass_plan_kernel(const View p, const Plan pl, int* base, int window, int first, int tq) {
+    rcu_kernel_entry();
+    __shared__ int warps[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int before = 0;
+    auto scan = [&](int w, int& at) {          // exclusive sum over the CTA, on top of `before`, which moves on
+        int upto = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 31) warps[warp] = upto;
+        __syncthreads();
+        int add = before, all = 0;
+        for (int j = 0; j < 32; ++j) {
+            if (j < warp) add += warps[j];
+            all += warps[j];
+        }
+        at = add + upto - w;
+        before += all;
+        __syncthreads();
+    };
+    for (int b = 0; b < p.S; b += 1024) {
+        int w = 0, at;
+        if (b + tid < p.S) {
+            const Seq q = seq_of(p, b + tid);
+            w = q.n > 0 ? (q.L + kTileK - 1) / kTileK : 0;
+        }
+        scan(w, at);
+        if (b + tid < p.S) base[b + tid] = at;
+    }
+    const int items = min(before, pl.items);
+    __syncthreads();                          // base is read by others
+    before = 0;
+    for (int b = 0; b < items; b += 1024) {
+        const int i = b + tid;
+        int w = 0, at;
+        if (i < items) {
+            int lo = 0, hi = p.S - 1;            // the last sequence with base <= i
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (base[mid] <= i) lo = mid;
+                else hi = mid - 1;
+            }
+            int j0, j1;
+            seen_by(seq_of(p, lo), window, first, tq, (i - base[lo]) * kTileK, j0, j1);
+            pl.item[i] = Item{lo, i - base[lo], j0, 0};
+            w = j1 - j0;
+        }
+        scan(w, at);
+        if (i < items) pl.prefix[i] = at;
+    }
+    if (tid == 0) {
+        pl.prefix[items] = before;
+        pl.head[0] = before;
+        const long long total = (long long)before * p.G;
+        pl.head[1] = (int)max(1ll, min((long long)pl.ctas, (total + pl.least - 1) / pl.least));
+        pl.head[2] = items;
+    }
+}
+
+struct MassArgs {
+    AttendArgs a;
+    Plan pl;
+    int group, tq, nb;
+};
+
+template <class T>
+__global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, MassArgs x) {
+    extern __shared__ unsigned char smem_dyn[];
+    const AttendArgs& a = x.a;
+    const View& p = a.p;
+    const int tile_bytes = x.nb * kBlock;
+    unsigned char* ks = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
+    unsigned char* ring = ks + 2 * tile_bytes;
+    __shared__ __align__(16) float lse[kStagesQ][kTileQ];
+    __shared__ __align__(16) int rows[kStagesQ][kTileQ];              // of the queries; -1: none
+    __shared__ float sums[2][kTileK];
+    __shared__ __align__(8) uint64_t k_full[2], k_empty[2], q_full[kStagesQ], q_empty[kStagesQ], s_full[4], s_empty[4], handed[2], taken[2], drained;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(&drained, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&handed[i], 4);
+            mbar_init(&taken[i], 4);
+        }
+        for (int i = 0; i < kStagesQ; ++i) {
+            mbar_init(&q_full[i], 33);
+            mbar_init(&q_empty[i], 5);           // the product's, and the four warps that read the lse
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_empty[i], 4);
+        }
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // rows of a query tile that no box fills
+    const int filled = x.tq * x.group;
+    for (int i = threadIdx.x; i < kStagesQ * x.nb * (kTileQ - filled) * 8; i += kThreadsM) {
+        const int block = i / ((kTileQ - filled) * 8), at = i % ((kTileQ - filled) * 8);
+        reinterpret_cast<uint4*>(ring + (size_t)block * kBlock + filled * 128)[at] = make_uint4(0, 0, 0, 0);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    rcu_kernel_entry_wait_only();        // nothing before this touches global memory
+    const uint32_t tmem = tmem_slot;
+    x.pl.items = x.pl.head[2];
+
+    if (warp == 0) {
+        const int rows_box = min(p.R, kTileK), boxes = kTileK / rows_box, box = lane % boxes, col = lane / boxes;
+        int item = 0, fills = 0;
+        bool ok = true;
+        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next(), ++item) {
+            const Seq q = seq_of(p, wk.it.s);
+            const int j0 = wk.it.token * kTileK, b = item & 1;
+            const int page = j0 + box * rows_box < q.L ? page_of(p, wk.it.s, j0 + box * rows_box) : -1;
+            const int pages = __popc(__ballot_sync(0xffffffffu, lane < boxes && page >= 0));
+            if (item >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[b], (item / 2 - 1) & 1, &abort_flag, p.status));
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(&k_full[b], pages * x.nb * rows_box * 128);
+            __syncwarp();
+            if (lane < boxes * x.nb && page >= 0) tma_load_4d(ks + b * tile_bytes + col * kBlock + box * rows_box * 128, &kmap, col * 64, j0 & (p.R - 1), wk.g, page, &k_full[b]);
+            for (int n = wk.n0; n < wk.n1 && ok; ++n, ++fills) {
+                const int s = fills % kStagesQ, t0 = (wk.it.count + n) * x.tq;
+                float v[4];
+                int r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int u = lane + 32 * i, t = t0 + u / x.group;
+                    const bool in = u < filled && t < q.n;
+                    v[i] = in ? a.lse[(size_t)(q.start + t) * a.H + wk.g * x.group + u % x.group] : INFINITY;
+                    r[i] = in ? q.old() + t : -1;
+                }
+                if (fills >= kStagesQ) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[s], (fills / kStagesQ - 1) & 1, &abort_flag, p.status));
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    lse[s][lane + 32 * i] = v[i];
+                    rows[s][lane + 32 * i] = r[i];
+                }
+                mbar_arrive(&q_full[s]);
+                if (lane == 0) {
+                    mbar_expect_tx(&q_full[s], x.nb * filled * 128);
+                    for (int c = 0; c < x.nb; ++c) tma_load_4d(ring + (size_t)s * tile_bytes + c * kBlock, &qmap, c * 64, 0, wk.g, q.start + t0, &q_full[s]);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {          // given up: let the copies in flight land before the memory is somebody else's
+            for (int i = max(0, fills - kStagesQ); i < fills; ++i)
+                for (int k = 0; k < (1 << 16) && !gemvq8::mbar_test_wait(&q_full[i % kStagesQ], (i / kStagesQ) & 1); ++k) {}
+            for (int i = max(0, item - 1); i <= item; ++i)
+                for (int k = 0; k < (1 << 16) && !gemvq8::mbar_test_wait(&k_full[i & 1], (i / 2) & 1); ++k) {}
+        }
+    } else if (warp == 1) {
+        constexpr bool bf16 = !std::is_same<T, __half>::value;
+        const uint32_t idesc = umma_idesc_f16(kTileK, kTileQ, bf16);
+        const int ksteps = (p.D + 15) / 16;
+        const uint64_t kd = umma_desc_sw128(ks), qd = umma_desc_sw128(ring);
+        const bool leader = elect_one();
+        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait_spin(bar, phase & 1, &abort_flag, p.status)); };
+        bool ok = true;
+        int item = 0, at = 0;                    // at: query tiles so far
+        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next(), ++item) {
+            const int b = item & 1;
+            ok = wait(&k_full[b], item / 2);
+            for (int n = wk.n0; n < wk.n1 && ok; ++n, ++at) {
+                const int s = at % kStagesQ, t = at & 3;
+                ok = wait(&q_full[s], at / kStagesQ);
+                if (ok && at >= 4) ok = wait(&s_empty[t], at / 4 - 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t ad = kd + (uint64_t)(b * (tile_bytes >> 4)), bd = qd + (uint64_t)(s * (tile_bytes >> 4));
+                    for (int k = 0; k < ksteps; ++k) {
+                        const uint64_t off = (k >> 2) * (kBlock >> 4) + 2 * (k & 3);
+                        umma_f16(tmem + 128 * t, ad + off, bd + off, idesc, k > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[t]);
+                    umma_commit(&q_empty[s]);
+                    if (n == wk.n1 - 1) umma_commit(&k_empty[b]);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok && leader) {            // given up: let the products in flight end before tensor memory is freed
+            umma_commit(&drained);
+            for (int i = 0; i < (1 << 20) && !gemvq8::mbar_test_wait(&drained, 0); ++i) {}
+        }
+        __syncwarp();
+    } else {
+        const int w = warp < 6 ? 0 : 1, quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait_spin(bar, phase & 1, &abort_flag, p.status)); };
+        bool ok = true;
+        int item = 0, at = 0;
+        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next(), ++item) {
+            const Seq q = seq_of(p, wk.it.s);
+            const int j0 = wk.it.token * kTileK, j = j0 + r;
+            float sum = 0.f;
+            for (int n = wk.n0; n < wk.n1 && ok; ++n, ++at) {
+                if ((at & 1) != w) continue;
+                const int s = at % kStagesQ, t = at & 3;
+                ok = wait(&q_full[s], at / kStagesQ) && wait(&s_full[t], at / 4);
+                if (!ok) break;
+                tc_fence_after();
+                const int t0 = (wk.it.count + n) * x.tq, r0 = q.old() + t0, r1 = r0 + x.tq - 1;
+                // every query sees every row of the tile
+                const bool whole = t0 + x.tq <= q.n && j0 + kTileK - 1 <= r0 && (a.window == 0 || j0 > r1 - a.window || j0 + kTileK <= a.first);
+                float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float z[64];
+                    tmem_ld_32x64(tmem + 128 * t + 64 * half + lanes, z);
+                    const float4* ls = reinterpret_cast<const float4*>(&lse[s][64 * half]);
+                    const int4* rs = reinterpret_cast<const int4*>(&rows[s][64 * half]);
+                    if (whole) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const float4 v = ls[c];
+                            add[0] += ex2(fmaf(z[4 * c], a.c, -v.x));
+                            add[1] += ex2(fmaf(z[4 * c + 1], a.c, -v.y));
+                            add[2] += ex2(fmaf(z[4 * c + 2], a.c, -v.z));
+                            add[3] += ex2(fmaf(z[4 * c + 3], a.c, -v.w));
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const float4 v = ls[c];
+                            const int4 at4 = rs[c];
+                            auto weight = [&](float score, float l, int row) {
+                                const bool in = j <= row && (a.window == 0 || j > row - a.window || j < a.first);
+                                return in ? ex2(fmaf(score, a.c, -l)) : 0.f;
+                            };
+                            add[0] += weight(z[4 * c], v.x, at4.x);
+                            add[1] += weight(z[4 * c + 1], v.y, at4.y);
+                            add[2] += weight(z[4 * c + 2], v.z, at4.z);
+                            add[3] += weight(z[4 * c + 3], v.w, at4.w);
+                        }
+                    }
+                }
+                sum += (add[0] + add[1]) + (add[2] + add[3]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&s_empty[t]);
+                    mbar_arrive(&q_empty[s]);
+                }
+            }
+            if (!ok) break;
+            // the second group's sums to the first: two places in turns
+            const int b = item & 1;
+            if (w == 1) {
+                if (item >= 2) ok = wait(&taken[b], item / 2 - 1);
+                if (!ok) break;
+                sums[b][r] = sum;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&handed[b]);
+            } else {
+                ok = wait(&handed[b], item / 2);
+                if (!ok) break;
+                sum += sums[b][r];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&taken[b]);
+                if (!wk.whole) reinterpret_cast<float*>(x.pl.ml)[wk.slot(blockIdx.x) * kTileK + r] = sum;
+                else if (j < q.L) p.mass[((size_t)wk.it.s * p.G + wk.g) * ((size_t)p.MP << p.shift) + j] += sum;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    }
+}
+
+// Adds the parts of tiles that several CTAs had, in their order (as merge_kernel).
+__global__ void __launch_bounds__(kTileK) mass_merge_kernel(const View p, Plan pl) {
+    rcu_kernel_entry();
+    const int W = pl.head[0], C = pl.head[1], b = blockIdx.x;
+    pl.items = pl.head[2];
+    if (b + 1 >= C) return;
+    const long long total = (long long)W * p.G;
+    const int begin = first_tile(total, b, C), cut = first_tile(total, b + 1, C);
+    Walk wk(pl, b + 1, p.G);
+    const int start = wk.g * W + pl.prefix[wk.i], stop = wk.g * W + pl.prefix[wk.i + 1];
+    if (start == cut || start < begin) return;
+    const float* parts = reinterpret_cast<const float*>(pl.ml);
+    const int r = threadIdx.x, j = wk.it.token * kTileK + r, L = clamp_int(p.lengths[wk.it.s], 0, p.MP << p.shift);
+    float sum = parts[(2 * b + (start != begin)) * kTileK + r];
+    for (int c = b + 1; c < C && first_tile(total, c, C) < stop; ++c) sum += parts[2 * c * kTileK + r];
+    if (j < L) p.mass[((size_t)wk.it.s * p.G + wk.g) * ((size_t)p.MP << p.shift) + j] += sum;
+}
+
+uint64_t mass_plan_of(const rcu_device* dev, const View& p, char* mem, Plan* out, int** base) {
+    Plan pl{};
+    pl.items = p.S * (((p.MP << p.shift) + kTileK - 1) / kTileK);
+    pl.ctas = dev->sm_count;
+    pl.least = 4;
+    uint64_t at = 0;
+    auto take = [&](uint64_t bytes) {
+        char* ptr = mem + at;
+        at += align256(bytes);
+        return ptr;
+    };
+    pl.head = (int*)take(12);
+    pl.prefix = (int*)take(4ull * (pl.items + 1));
+    pl.item = (Item*)take(sizeof(Item) * (uint64_t)pl.items);
+    pl.ml = (float2*)take(4ull * 2 * pl.ctas * kTileK);
+    int* b = (int*)take(4ull * p.S);
+    if (out) *out = pl;
+    if (base) *base = b;
+    return at;
+}
+
+template <class T> rcu_status launch_mass(rcu_device* dev, const AttendArgs& a, int dt, void* scratch) {
+    const View& p = a.p;
+    MassArgs x{a, {}, a.H / p.G, kTileQ / (a.H / p.G), (p.D + 63) / 64};
+    int* base;
+    mass_plan_of(dev, p, (char*)scratch, &x.pl, &base);
+    CUtensorMap qm, km;
+    if (!map_queries(&qm, dt, p, a.q, x.group, x.tq) || !map_pages(&km, dt, p, p.keys, p.D))
+        return rcu_fail(dev, RCU_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (%d tokens, %d heads, %d pages)", p.T, a.H, p.pages);
+    rcu_launch(dev, mass_plan_kernel, 1, 1024, 0, p, x.pl, base, a.window, a.first, x.tq);
+    RCU_LAUNCH_CHECK(dev);
+    const size_t smem = 1024 + (size_t)(2 + kStagesQ) * x.nb * kBlock;
+    void (*kern)(CUtensorMap, CUtensorMap, MassArgs) = mass_tc_kernel<T>;
+    RCU_CUDA(dev, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    RCU_CUDA(dev, rcu_launch(dev, kern, x.pl.ctas, kThreadsM, smem, qm, km, x));
+    RCU_LAUNCH_CHECK(dev);
+    if (x.pl.ctas > 1) {
+        rcu_launch(dev, mass_merge_kernel, x.pl.ctas - 1, kTileK, 0, p, x.pl);
+        RCU_LAUNCH_CHECK(dev);
+    }
+    return RCU_OK;
+}
+
+}  // namespace
+
+uint64_t mass_tc_scratch(const rcu_device* dev, const View& p, int) { return mass_plan_of(dev, p, nullptr, nullptr, nullptr); }
+
+rcu_status mass_tc(rcu_device* dev, const AttendArgs& a, int dt, void* scratch) {
+    return dt == RCU_BF16 ? launch_mass<__nv_bfloat16>(dev, a, dt, scratch) : launch_mass<__half>(dev, a, dt, scratch);
+}
+
+}  // namespace paged
