@@ -70,11 +70,11 @@ __device__ __forceinline__ int first_tile(long long total, int b, int C) { retur
 // A CTA's walk over its run: item by item
 struct Walk {
     const Plan& pl;
-    int W, at, end, begin;     // tiles of a kv head; run
+    int items, W, at, end, begin;     // items and tiles of a kv head; run
     int g, i;                  // kv head and item at `at`
     Item it;
     int n0, n1, whole;         // tiles [n0, n1) of the item; whether these are all of them
-    __device__ __forceinline__ Walk(const Plan& plan, int b, int G) : pl(plan) {
+    __device__ __forceinline__ Walk(const Plan& plan, int b, int G, int count) : pl(plan), items(count) {
         W = plan.head[0];
         const int C = plan.head[1];
         const long long total = (long long)W * G;
@@ -85,7 +85,7 @@ struct Walk {
     __device__ __forceinline__ void find() {
         g = at / W;
         const int y = at - g * W;
-        int lo = 0, hi = pl.items - 1;                  // the last item with prefix <= y
+        int lo = 0, hi = items - 1;                  // the last item with prefix <= y
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
             if (pl.prefix[mid] <= y) lo = mid;

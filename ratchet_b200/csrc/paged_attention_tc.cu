@@ -6,8 +6,10 @@
 //                       rows of no page stay as they are in shared memory);
 //   warp 1              per tile n and query tile w: O_w += P_w V of tile n - 1, with P_w read from tensor memory, then S_w = Q_w K^T of tile n,
 //                       which takes P_w's place;
-//   warps 2-5, 6-9      softmax of tile 0 / 1, a query per thread: scores from tensor memory, mask, running maximum, weights back over the scores.
-//                       The maximum that weights are taken against only moves when a score exceeds it by more than 2^8, so that O_w is rescaled rarely.
+//   warps 4-7, 8-11     softmax of query tile 0 / 1, a query per thread: scores from tensor
+//                       memory, mask, running maximum, weights back over the scores in two halves.  The maximum that weights are taken against
+//                       only moves when a score exceeds it by more than 2^8, so that O_w is rescaled rarely.
+// An item of one query tile (generation) gives it to both groups, which take the tiles of rows in turns and join their sums at the end.
 // Weights enter the second product in the operands' type: half a step of theirs moves the sum by as much as the rounding of the output does.  Their
 // sum, the maximum and O are f32.
 // What is masked must not reach the sum even where it is not finite, and 0 times infinity is NaN.  Rows behind the sequence's last one are zeroed in
@@ -23,17 +25,8 @@
 namespace paged {
 namespace {
 
-constexpr int kThreadsP = 320, kMostStages = 8;
+constexpr int kThreadsP = 384, kMostStages = 8;
 
-template <class T> __device__ __forceinline__ uint32_t pack2(float x, float y);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
-    const __half2 v = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 // whether one of the two 16-bit values is an infinity or NaN
 template <class T> __device__ __forceinline__ uint32_t not_finite(uint32_t x);
 template <> __device__ __forceinline__ uint32_t not_finite<__half>(uint32_t x) { return __vcmpgeu2(x & 0x7fff7fffu, 0x7c007c00u); }
@@ -99,15 +92,63 @@ struct TcArgs {
     int stages, nb, eb, stage_bytes;
 };
 
+// Which tiles of an item's span (by their place in it) some query at rows t0 .. t1 sees
+struct Sight {
+    int head, a, b;
+    __device__ __forceinline__ bool operator()(int n) const { return n < head || (n >= a && n < b); }
+};
+__device__ __forceinline__ Sight sight_of(int window, int first, const Span& sp, int t0, int t1) {
+    Sight v{0, 0, 0};
+    if (t1 < t0 || t1 < 0) return v;
+    const int low = window > 0 ? max(0, t0 - window + 1) : 0;
+    v.head = window > 0 ? (sp.head > 0 ? sp.head : (min(first, t1 + 1) + kTileK - 1) / kTileK) : 0;
+    v.a = max(low / kTileK - sp.lo, 0) + sp.head;
+    v.b = t1 / kTileK + 1 - sp.lo + sp.head;
+    return v;
+}
+
+// A CTA's share of an item, as one warp works it out for the others
+struct alignas(16) Segment {
+    Item it;
+    int g, n0, n1, slot;
+    int whole, more, L, two;             // more 0: the run has ended; two: the item has a second query tile
+    Span sp;
+    Sight see[2];
+    int pad[3];
+    // An item of two query tiles: group w has tile w.  Of one: both groups have it, the tiles of rows in turns.
+    __device__ __forceinline__ bool has(int w, int n) const { return see[w](n) && (two || ((n - n0) & 1) == w); }
+};
+constexpr int kSegments = 4;
+
+// A query tile whose values are not all finite, row by row
+template <class T>
+__device__ __noinline__ void redo_rows(const TcArgs& x, const Segment& seg, int w, int quarter) {
+    const int tile0 = seg.two ? w * x.tq : 0;
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+        const int r = quarter * 32 + i, t = tile0 + r / x.group, h = seg.g * x.group + r % x.group;
+        if (r >= x.tq * x.group || t >= seg.it.count) continue;
+        RowPart part;
+        attend_row<T>(x.a, seg.it.s, seg.g, seg.it.token + t, h, seg.it.row + t, seg.sp, seg.n0, seg.n1, part);
+        if (seg.whole) finish_row<T>(x.a, seg.it.token + t, h, part);
+        else store_part(x.pl, x.a.p.E, seg.slot, (seg.two ? w : 0) * kTileQ + r, part);
+    }
+}
+
 template <class T>
 __global__ void __launch_bounds__(kThreadsP, 1)
-paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const TcArgs x) {
+paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                const __grid_constant__ TcArgs x) {
     extern __shared__ unsigned char smem_dyn[];
     const AttendArgs& a = x.a;
     const View& p = a.p;
     unsigned char* qs = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
     unsigned char* ring = qs + 2 * x.nb * kBlock;
-    __shared__ __align__(8) uint64_t q_full, q_empty, full[kMostStages], empty[kMostStages], s_full[2], p_full[2], o_full[2], met[2], drained;
+    // p_full: a half of the tile's rows each, so that the product with V begins while the second half's weights are worked out
+    __shared__ __align__(8) uint64_t q_full, q_empty, full[kMostStages], empty[kMostStages], s_full[2], p_full[2][2], o_full[2], met[2], joined, taken, drained,
+        seg_full[kSegments], seg_empty[kSegments];
+    __shared__ Segment segments[kSegments];
+    __shared__ float2 other[kTileQ];                  // maximum and sum that the second group hands to the first
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag, poison[2];
 
@@ -115,14 +156,24 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
         mbar_init(&q_empty, 1);
+        mbar_init(&joined, 8);
+        mbar_init(&taken, 4);
         mbar_init(&drained, 1);
+#pragma unroll 1
         for (int i = 0; i < x.stages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
+#pragma unroll 1
+        for (int i = 0; i < kSegments; ++i) {
+            mbar_init(&seg_full[i], 1);
+            mbar_init(&seg_empty[i], 10);
+        }
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i][0], 4);
+            mbar_init(&p_full[i][1], 4);
             mbar_init(&o_full[i], 1);
             mbar_init(&met[i], 4);
             poison[i] = 0;
@@ -140,285 +191,423 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
     rcu_kernel_entry_wait_only();        // nothing before this touches global memory
     const uint32_t tmem = tmem_slot;       // S_w (then P_w) at 128 w, O_w at 256 + 128 w
 
-    // whether query tile w of an item sees any of the rows j0 .. j0 + 127; the item's tokens are at rows row .. row + count - 1
-    auto sees = [&](const Item& it, int w, int j0) {
-        const int r0 = it.row + w * x.tq, r1 = min(r0 + x.tq, it.row + it.count) - 1;
-        return r0 <= r1 && j0 <= r1 && (a.window == 0 || j0 + kTileK - 1 > r0 - a.window || j0 < a.first);
+    auto wait = [&](uint64_t* bar, int phase) { return wait_warp(bar, phase, &abort_flag, p.status); };
+    // The i-th segment; false where the run has ended, or a wait gave up (ok)
+    auto take = [&](int i, bool& ok) -> const Segment& {
+        ok = wait(&seg_full[i % kSegments], i / kSegments);
+        return segments[i % kSegments];
     };
-    auto spans = [&](const Item& it) { return span_of(a.window, a.first, it.row, it.row + it.count - 1); };
+    auto release = [&](int i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_empty[i % kSegments]);
+    };
 
-    if (warp == 0) {
+    if (warp == 2) {
+        Walk wk(x.pl, blockIdx.x, p.G, x.pl.items);
+        bool ok = true;
+#pragma unroll 1
+        for (int i = 0; ok; ++i) {
+            ok = wait(&seg_empty[i % kSegments], (i / kSegments) ^ 1);
+            if (!ok) break;
+            const bool more = wk.more();
+            Segment& seg = segments[i % kSegments];
+            if (lane == 0) {
+                seg.more = more;
+                if (more) {
+                    const Span sp = span_of(a.window, a.first, wk.it.row, wk.it.row + wk.it.count - 1);
+                    const bool two = wk.it.count > x.tq;
+                    seg.it = wk.it;
+                    seg.g = wk.g;
+                    seg.n0 = wk.n0;
+                    seg.n1 = wk.n1;
+                    seg.slot = wk.slot(blockIdx.x);
+                    seg.whole = wk.whole;
+                    seg.L = clamp_int(p.lengths[wk.it.s], 0, p.MP << p.shift);
+                    seg.two = two;
+                    seg.sp = sp;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const int t0 = wk.it.row + (two ? w * x.tq : 0);
+                        seg.see[w] = sight_of(a.window, a.first, sp, t0, min(t0 + x.tq, wk.it.row + wk.it.count) - 1);
+                    }
+                }
+                mbar_arrive(&seg_full[i % kSegments]);
+            }
+            __syncwarp();
+            if (!more) break;
+            wk.next();
+        }
+    } else if (warp == 0) {
         const int rows_box = min(p.R, kTileK), boxes = kTileK / rows_box;
         const bool mine_k = lane < boxes * x.nb, mine_v = lane < boxes * x.eb;
         const int box = lane % boxes, col = lane / boxes;
-        int fills = 0, seg = 0;
+        int fills = 0, i = 0;
+        RingAt at{x.stages, 0, 0};
         bool ok = true;
-        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next(), ++seg) {
-            const Span sp = spans(wk.it);
-            const int L = clamp_int(p.lengths[wk.it.s], 0, p.MP << p.shift);
-            const bool second = wk.it.count > x.tq;
-            if (seg > 0) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty, (seg - 1) & 1, &abort_flag, p.status));
+#pragma unroll 1
+        for (;; ++i) {
+            const Segment& seg = take(i, ok);
+            if (!ok || !seg.more) break;
+            ok = wait(&q_empty, i ^ 1);
             if (!ok) break;
             if (lane == 0) {
-                const int tiles = second ? 2 : 1;
+                const int tiles = seg.two ? 2 : 1;
                 mbar_expect_tx(&q_full, tiles * x.nb * x.group * x.tq * 128);
-                for (int w = 0; w < tiles; ++w)
-                    for (int b = 0; b < x.nb; ++b) tma_load_4d(qs + (w * x.nb + b) * kBlock, &qmap, b * 64, 0, wk.g, wk.it.token + w * x.tq, &q_full);
+#pragma unroll 1
+                for (int w = 0; w < tiles * x.nb; ++w)
+                    tma_load_4d(qs + w * kBlock, &qmap, w % x.nb * 64, 0, seg.g, seg.it.token + w / x.nb * x.tq, &q_full);
             }
             __syncwarp();
-            auto page_at = [&](int n) {          // of this lane's box; -1 behind the last row
-                const int j = sp.tile(n) * kTileK + box * rows_box;
-                return j < L ? page_of(p, wk.it.s, j) : -1;
-            };
-            int page = page_at(wk.n0);
-            for (int n = wk.n0; n < wk.n1 && ok; ++n) {
-                const int j0 = sp.tile(n) * kTileK, at = j0 & (p.R - 1);
-                const int next = n + 1 < wk.n1 ? page_at(n + 1) : -1;
-                const int pages = __popc(__ballot_sync(0xffffffffu, lane < boxes && page >= 0));
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv, ++fills) {
-                    const int s = fills % x.stages;
-                    if (fills >= x.stages) ok = ok && __all_sync(0xffffffffu, mbar_wait(&empty[s], (fills / x.stages - 1) & 1, &abort_flag, p.status));
+            PageIds ids;
+            const int L = seg.L, have = min(p.MP, (L + p.R - 1) >> p.shift);
+#pragma unroll 1
+            for (int n = seg.n0; n < seg.n1 && ok; ++n) {
+                const int j0 = seg.sp.tile(n) * kTileK, i0 = j0 >> p.shift, row0 = j0 & (p.R - 1);
+                const bool in = j0 + box * rows_box < L;               // boxes behind the last row are left out
+                const int page = ids.of(p, seg.it.s, i0, i0 + box, i0 + boxes - 1, have);
+                const int pages = min(boxes, (L - j0 + rows_box - 1) / rows_box);
+#pragma unroll 1
+                for (int kv = 0; kv < 2; ++kv) {
+                    ok = wait(&empty[at.s], at.phase ^ 1);
                     if (!ok) break;
-                    const int blocks = kv ? x.eb : x.nb;
-                    if (lane == 0) mbar_expect_tx(&full[s], pages * blocks * rows_box * 128);
+                    if (lane == 0) mbar_expect_tx(&full[at.s], pages * (kv ? x.eb : x.nb) * rows_box * 128);
                     __syncwarp();
-                    if ((kv ? mine_v : mine_k) && page >= 0)
-                        tma_load_4d(ring + (size_t)s * x.stage_bytes + col * kBlock + box * rows_box * 128, kv ? &vmap : &kmap, col * 64, at, wk.g, page, &full[s]);
+                    if ((kv ? mine_v : mine_k) && in)
+                        tma_load_4d(ring + (size_t)at.s * x.stage_bytes + col * kBlock + box * rows_box * 128, kv ? &vmap : &kmap, col * 64, row0, seg.g, page, &full[at.s]);
+                    at.go(1);
+                    ++fills;
                 }
-                page = next;
             }
+            if (!ok) break;
+            release(i);
         }
         if (!ok) {          // given up: let the copies in flight land before the memory is somebody else's
-            for (int i = max(0, fills - x.stages); i < fills; ++i)
-                for (int k = 0; k < (1 << 16) && !gemvq8::mbar_test_wait(&full[i % x.stages], (i / x.stages) & 1); ++k) {}
-            for (int k = 0; k < (1 << 16) && !gemvq8::mbar_test_wait(&q_full, seg & 1); ++k) {}
+#pragma unroll 1
+            for (int k = max(0, fills - x.stages); k < fills; ++k) land(&full[k % x.stages], k / x.stages);
+            land(&q_full, i);
         }
     } else if (warp == 1) {
         // the whole warp keeps step, one elected lane issues
-        constexpr bool bf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+        constexpr bool bf16 = !std::is_same<T, __half>::value;
         const uint32_t idesc_s = umma_idesc_f16(kTileQ, kTileK, bf16);
         const uint32_t idesc_o = umma_idesc_f16(kTileQ, (p.E + 15) & ~15, bf16) | (1u << 16);     // V is stored with its columns contiguous
         const int ksteps = (p.D + 15) / 16;
         const uint64_t qd = umma_desc_sw128(qs), kd = umma_desc_sw128(ring), vd = umma_desc_sw128_mn(ring, kBlock);
         const bool leader = elect_one();
-        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait_spin(bar, phase & 1, &abort_flag, p.status)); };
         bool ok = true;
-        int seg = 0, base = 0, weights[2] = {0, 0};          // base: fills before this run; weights: hand-overs of P_w so far
-        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next(), ++seg) {
-            const Span sp = spans(wk.it);
-            const int count = wk.n1 - wk.n0;
-            bool any[2] = {false, false};
-            ok = wait(&q_full, seg);
-            for (int m = 0; m <= count && ok; ++m) {
-                const int kf = base + 2 * m, vf = base + 2 * m - 1;          // fills of K of this tile, V of the one before
-                const int j0 = m < count ? sp.tile(wk.n0 + m) * kTileK : 0, i0 = m > 0 ? sp.tile(wk.n0 + m - 1) * kTileK : 0;
-                if (m < count) ok = wait(&full[kf % x.stages], kf / x.stages);
-                if (ok && m > 0) ok = wait(&full[vf % x.stages], vf / x.stages);
+        int weights0 = 0, weights1 = 0;                // hand-overs of P_w so far
+        RingAt kat{x.stages, 0, 0}, vat{x.stages, 1, 0};
+#pragma unroll 1
+        for (int i = 0;; ++i) {
+            const Segment& seg = take(i, ok);
+            if (!ok || !seg.more) break;
+            const int n0 = seg.n0, n1 = seg.n1;
+            const bool two = seg.two;
+            bool any0 = false, any1 = false;
+            ok = wait(&q_full, i);
+#pragma unroll 1
+            for (int n = n0; n <= n1 && ok; ++n) {
+                const bool last = n == n1;
+                const uint64_t kb = kd + (uint64_t)(kat.s * (x.stage_bytes >> 4)), vb = vd + (uint64_t)(vat.s * (x.stage_bytes >> 4));
+                auto scores = [&](auto w) {
+                    if (last || !seg.has(w, n)) return;
+                    tc_fence_after();
+                    if (leader) {
+                        const uint64_t qa = qd + (uint64_t)((two ? w() : 0) * x.nb * (kBlock >> 4));
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    if (ok && m > 0 && sees(wk.it, w, i0)) {
-                        ok = wait(&p_full[w], weights[w]++);
+                        for (int k = 0; k < 8; ++k)
+                            if (k < ksteps) umma_f16(tmem + 128 * w, qa + (k >> 2) * (kBlock >> 4) + 2 * (k & 3), kb + (k >> 2) * (kBlock >> 4) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
+                        umma_commit(&s_full[w]);
+                    }
+                    __syncwarp();
+                };
+                auto values = [&](auto w, int& weights, bool& any) {
+                    if (n == n0 || !seg.has(w, n - 1)) return;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (ok) ok = wait(&p_full[w][half], weights);
                         tc_fence_after();
                         if (ok && leader) {
-                            const uint64_t bd = vd + (uint64_t)((vf % x.stages) * (x.stage_bytes >> 4));
 #pragma unroll
-                            for (int k = 0; k < kTileK / 16; ++k)      // 16 rows are two 1024-byte groups of V, eight columns of P
-                                umma_f16_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * k, bd + 128 * k, idesc_o, k > 0 || any[w] ? 1u : 0u);
-                        }
-                        any[w] = true;
-                        __syncwarp();
-                    }
-                    if (ok && m < count && sees(wk.it, w, j0)) {
-                        tc_fence_after();
-                        if (leader) {
-                            const uint64_t ad = qd + (uint64_t)(w * x.nb * (kBlock >> 4)), bd = kd + (uint64_t)((kf % x.stages) * (x.stage_bytes >> 4));
-                            for (int k = 0; k < ksteps; ++k) {
-                                const uint64_t off = (k >> 2) * (kBlock >> 4) + 2 * (k & 3);
-                                umma_f16(tmem + 128 * w, ad + off, bd + off, idesc_s, k > 0 ? 1u : 0u);
-                            }
-                            umma_commit(&s_full[w]);
+                            for (int k = 4 * half; k < 4 * half + 4; ++k)      // 16 rows are two 1024-byte groups of V, eight columns of P
+                                umma_f16_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * k, vb + 128 * k, idesc_o, k > 0 || any ? 1u : 0u);
                         }
                         __syncwarp();
                     }
+                    ++weights;
+                    any = true;
+                };
+                using W0 = std::integral_constant<int, 0>;
+                using W1 = std::integral_constant<int, 1>;
+                if (!last) ok = wait(&full[kat.s], kat.phase);
+                if (!ok) break;
+                // in turns, the two groups' tiles are different ones: the scores of one need not wait for the weights of the other
+                if (!two) {
+                    scores(W0{});
+                    scores(W1{});
                 }
+                if (n > n0) ok = wait(&full[vat.s], vat.phase);
+                if (ok) values(W0{}, weights0, any0);
+                if (ok && two) scores(W0{});
+                if (ok) values(W1{}, weights1, any1);
+                if (ok && two) scores(W1{});
                 if (!ok) break;
                 if (leader) {
-                    if (m < count) umma_commit(&empty[kf % x.stages]);
-                    if (m == count - 1) umma_commit(&q_empty);
-                    if (m > 0) umma_commit(&empty[vf % x.stages]);
-                    if (m == count) {
-                        if (any[0]) umma_commit(&o_full[0]);
-                        if (any[1]) umma_commit(&o_full[1]);
-                    }
+                    if (!last) umma_commit(&empty[kat.s]);
+                    if (n == n1 - 1) umma_commit(&q_empty);
+                    if (n > n0) umma_commit(&empty[vat.s]);
+                    if (last && any0) umma_commit(&o_full[0]);
+                    if (last && any1) umma_commit(&o_full[1]);
                 }
                 __syncwarp();
+                if (!last) kat.go(2);
+                if (n > n0) vat.go(2);
             }
-            base += 2 * count;
+            if (!ok) break;
+            release(i);
         }
         if (!ok && leader) {            // given up: let the products in flight end before tensor memory is freed
             umma_commit(&drained);
-            for (int i = 0; i < (1 << 20) && !gemvq8::mbar_test_wait(&drained, 0); ++i) {}
+            for (int k = 0; k < 16; ++k) land(&drained, 0);
         }
         __syncwarp();
-    } else {
-        const int w = warp < 6 ? 0 : 1, quarter = warp & 3;
+    } else if (warp >= 4) {
+        const int w = warp < 8 ? 0 : 1, quarter = warp & 3;
         const int r = quarter * 32 + lane;                                   // row of the query tile
-        const int token = w * x.tq + r / x.group, head = r % x.group;        // token of the item, query head of the group
+        const int own = r / x.group, head = r - own * x.group;               // token of the tile, query head of the group
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, ts = tmem + 128 * w + lanes, to = tmem + 256 + 128 * w + lanes;
         const int ocols = (p.E + 31) & ~31;
-        int base = 0, scores = 0, outs = 0, meets = 0;
+        uint4* turn = reinterpret_cast<uint4*>(ring + (size_t)x.stages * x.stage_bytes) + (warp - 4) * 128;      // 32 rows of 64 bytes, the warp's own
+        int scores = 0, outs = 0, meets = 0, joins = 0;
+        RingAt vat{x.stages, 1, 0};
         bool ok = true;
-        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait_spin(bar, phase & 1, &abort_flag, p.status)); };
-        auto meet = [&]() {              // the tile's four warps; bounded like every wait
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&met[w]);
-            return wait(&met[w], meets++);
-        };
-        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next()) {
-            const Span sp = spans(wk.it);
-            const int L = clamp_int(p.lengths[wk.it.s], 0, p.MP << p.shift);
-            const bool valid = r < x.tq * x.group && token < wk.it.count;
-            const int row = wk.it.row + token;
+#pragma unroll 1
+        for (int i = 0;; ++i) {
+            const Segment& seg = take(i, ok);
+            if (!ok || !seg.more) break;
+            const bool two = seg.two;
+            const Item it = seg.it;
+            const int tile0 = two ? w * x.tq : 0, token = tile0 + own, L = seg.L, n1 = seg.n1;
+            const bool valid = r < x.tq * x.group && token < it.count;
+            const int row = it.row + token;
             const bool live = __any_sync(0xffffffffu, valid);               // warps without a query only keep step
             // rows of the tile's and of the warp's first and last query
-            const int t0 = wk.it.row + w * x.tq, t1 = min(t0 + x.tq, wk.it.row + wk.it.count) - 1;
+            const int t0 = it.row + tile0, t1 = min(t0 + x.tq, it.row + it.count) - 1;
             const int w0 = __reduce_min_sync(0xffffffffu, valid ? row : 0x7fffffff), w1 = __reduce_max_sync(0xffffffffu, valid ? row : -1);
             float m = valid ? -INFINITY : INFINITY, l = 0.f;                // a row of no query never moves the maximum
             bool any = false;
-            for (int n = wk.n0; n < wk.n1 && ok; ++n) {
-                const int j0 = sp.tile(n) * kTileK, vf = base + 2 * (n - wk.n0) + 1;
-                if (!sees(wk.it, w, j0)) continue;
+#pragma unroll 1
+            for (int n = seg.n0; n < n1; ++n, vat.go(2)) {
+                if (!seg.has(w, n)) continue;
+                const int j0 = seg.sp.tile(n) * kTileK;
                 // a tile that is not whole to all queries: rows behind the last one become zero, values that are not finite are noted
-                const bool part = j0 + kTileK - 1 > t0 || (a.window > 0 && j0 <= t1 - a.window && j0 + kTileK > a.first);
-                if (part) {
-                    ok = wait(&full[vf % x.stages], vf / x.stages);
+                if (j0 + kTileK - 1 > t0 || (a.window > 0 && j0 <= t1 - a.window && j0 + kTileK > a.first)) {
+                    ok = wait(&full[vat.s], vat.phase);
                     if (!ok) break;
-                    unsigned char* v = ring + (size_t)(vf % x.stages) * x.stage_bytes + r * 128;
+                    unsigned char* v = ring + (size_t)vat.s * x.stage_bytes + r * 128;
                     const bool behind = j0 + r >= L;
                     uint32_t bad = 0;
-                    for (int b = 0; b < x.eb; ++b)
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            uint4* at = reinterpret_cast<uint4*>(v + b * kBlock + ((c ^ (lane & 7)) << 4));
-                            if (behind) *at = make_uint4(0, 0, 0, 0);
-                            else {
-                                const uint4 u = *at;
-                                bad |= not_finite<T>(u.x) | not_finite<T>(u.y) | not_finite<T>(u.z) | not_finite<T>(u.w);
-                            }
-                        }
+#pragma unroll 4
+                    for (int c = 0; c < 8 * x.eb; ++c) {
+                        uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * kBlock + (((c ^ lane) & 7) << 4));
+                        const uint4 u = *at;
+                        if (behind) *at = make_uint4(0, 0, 0, 0);
+                        else bad |= not_finite<T>(u.x) | not_finite<T>(u.y) | not_finite<T>(u.z) | not_finite<T>(u.w);
+                    }
                     if (bad) poison[w] = 1;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 ok = wait(&s_full[w], scores++);
                 if (!ok) break;
                 tc_fence_after();
-                if (live) {
-                    float s[128];
-                    tmem_ld_32x64(ts, s);
-                    tmem_ld_32x64(ts + 64, s + 64);
-                    if (j0 + kTileK - 1 > w0 || (a.window > 0 && j0 <= w1 - a.window && j0 + kTileK > a.first)) {
-                        const int hi = row - j0, lo = a.window > 0 ? hi - a.window : -1, head_end = a.first - j0;
+                auto hand_over = [&](int half) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[w][half]);
+                };
+                if (!live) {
+                    hand_over(0);
+                    hand_over(1);
+                    any = true;
+                    continue;
+                }
+                // 32 columns at a time, read twice (masked ones are written back the first time): tensor memory gives them in 70 cycles, and loops of a
+                // few kilobytes stay in the instruction cache
+                const bool masked = j0 + kTileK - 1 > w0 || (a.window > 0 && j0 <= w1 - a.window && j0 + kTileK > a.first);
+                float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float s[32];
+                    tmem_ld_32x32(ts + 32 * c, s);
+                    if (masked) {
+                        const int hi = row - j0 - 32 * c, lo = a.window > 0 ? hi - a.window : -1, head_end = a.first - j0 - 32 * c;
 #pragma unroll
-                        for (int j = 0; j < 128; ++j)
+                        for (int j = 0; j < 32; ++j)
                             if (j > hi || (j <= lo && j >= head_end)) s[j] = -INFINITY;
+                        tmem_st_32x32(ts + 32 * c, reinterpret_cast<const uint32_t*>(s));
                     }
-                    float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int j = 4; j < 128; ++j) top4[j & 3] = fmaxf(top4[j & 3], s[j]);
-                    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * a.c;      // c > 0
-                    const bool move = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
-                    const float next = move ? top : m;
-                    const float corr = move ? ex2(m - next) : 1.f;                    // 0 while no key has been seen
-                    m = next;
-                    const float z = m == -INFINITY ? 0.f : -m;
-                    float l4[4] = {l * corr, 0.f, 0.f, 0.f};
-                    uint32_t pw[64];
+                    for (int j = 0; j < 32; j += 8)
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) {
-                        const float u = ex2(fmaf(s[2 * j], a.c, z)), v = ex2(fmaf(s[2 * j + 1], a.c, z));
-                        l4[j & 3] += u + v;
-                        pw[j] = pack2<T>(u, v);
+                        for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], s[j + e], s[j + 4 + e]);
+                }
+                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * a.c;      // c > 0
+                const bool move = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
+                const float next = move ? top : m;
+                const float corr = move ? ex2(m - next) : 1.f;                    // 0 while no key has been seen
+                m = next;
+                const float z = m == -INFINITY ? 0.f : -m;
+                // the scores came behind the product of the tile before with V: O may be rescaled
+                if (any && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                    for (int c = 0; c < ocols; c += 32) {
+                        float o[32];
+                        tmem_ld_32x32(to + c, o);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] *= corr;
+                        tmem_st_32x32(to + c, reinterpret_cast<const uint32_t*>(o));
                     }
-                    l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                    // the scores came behind the tile before's product with V: O may be rescaled
-                    if (any && __any_sync(0xffffffffu, move)) {
-                        for (int c = 0; c < ocols; c += 32) {
-                            float o[32];
-                            tmem_ld_32x32(to + c, o);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] *= corr;
-                            tmem_st_32x32(to + c, reinterpret_cast<const uint32_t*>(o));
-                        }
-                    }
-                    tmem_st_32x64(ts, pw);
                 }
                 any = true;
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[w]);
+                const float2 c2 = make_float2(a.c, a.c), z2 = make_float2(z, z);
+                float2 l4[4] = {make_float2(l * corr, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                auto weigh = [&](const float (&s)[32], int c) {
+                    uint32_t pw[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 t = fma2(make_float2(s[2 * j], s[2 * j + 1]), c2, z2);
+                        // every fourth pair on the FMA pipe, which takes that off the exponential unit
+                        const float2 u = (j & 3) == 3 ? ex2_fma(t) : make_float2(ex2(t.x), ex2(t.y));
+                        l4[j & 3] = add2(l4[j & 3], u);
+                        pw[j] = pack2<T>(u.x, u.y);
+                    }
+                    tmem_st_32x16_start(ts + 16 * c, pw);          // over columns that have been read
+                };
+                float s0[32], s1[32];
+                tmem_ld_32x32_start(ts, s0);
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    tmem_ld_wait();
+                    tmem_ld_32x32_start(ts + 64 * half + 32, s1);
+                    weigh(s0, 2 * half);
+                    tmem_ld_wait();
+                    if (half == 0) tmem_ld_32x32_start(ts + 64, s0);
+                    weigh(s1, 2 * half + 1);
+                    tmem_st_wait();
+                    hand_over(half);
+                }
+                const float2 lb = add2(add2(l4[0], l4[1]), add2(l4[2], l4[3]));
+                l = lb.x + lb.y;
             }
             if (!ok) break;
-            base += 2 * (wk.n1 - wk.n0);
             if (any) {
                 ok = wait(&o_full[w], outs++);
                 if (!ok) break;
                 tc_fence_after();
+            } else if (valid) {
+                m = -INFINITY;
             }
-            const int slot = wk.slot(blockIdx.x), part_row = w * kTileQ + r;
-            const int h = wk.g * x.group + head;
-            const size_t q_at = (size_t)(wk.it.token + token) * a.H + h;
-            ok = meet();
+            // all of the tile's warps, or of both groups where these join their sums
+            if (!two && w == 1) other[r] = make_float2(m, l);
+            tc_fence_before();
+            uint64_t* bar = two ? &met[w] : &joined;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+            ok = wait(bar, two ? meets++ : joins);
             if (!ok) break;
-            if (poison[w]) {
-                if (live)
-                    for (int i = 0; i < 32; ++i) {
-                        const int ri = quarter * 32 + i, ti = w * x.tq + ri / x.group;
-                        if (ri >= x.tq * x.group || ti >= wk.it.count) continue;
-                        RowPart part;
-                        attend_row<T>(a, wk.it.s, wk.g, wk.it.token + ti, wk.g * x.group + ri % x.group, wk.it.row + ti, sp, wk.n0, wk.n1, part);
-                        if (wk.whole) finish_row<T>(a, wk.it.token + ti, wk.g * x.group + ri % x.group, part);
-                        else store_part(x.pl, p.E, slot, w * kTileQ + ri, part);
-                    }
-                ok = meet();
+            tc_fence_after();
+            if (!two && w == 1) {
+                ok = wait(&taken, joins++);
                 if (!ok) break;
-                poison[w] = 0;
-                ok = meet();
-            } else if (live) {
-                float inv = 1.f;
-                if (wk.whole) {
-                    if (a.sink && valid) l += ex2(a.sink[h] * kLog2e - m);
-                    inv = valid && any && row >= 0 ? 1.f / l : 0.f;
-                    if (a.lse && valid) a.lse[q_at] = m + log2f(l);
-                } else if (valid) {
-                    x.pl.ml[(size_t)slot * x.pl.stride + part_row] = make_float2(any ? m : -INFINITY, l);
+                release(i);
+                continue;
+            }
+            float scale0 = 1.f, scale1 = 0.f;                         // of this group's O and, where it joins the two, of the other's
+            bool both = false;                                        // whether the other group has had a tile
+            if (!two) {
+                const float2 ml = other[r];
+                const float t = fmaxf(m, ml.x);
+                if (t > -INFINITY) {
+                    scale0 = ex2(m - t);
+                    scale1 = ex2(ml.x - t);
                 }
-                if (any) {
-                    T* out = (T*)a.out + q_at * p.E;
-                    float4* parts = x.pl.o + (size_t)slot * (p.E / 4) * x.pl.stride + part_row;
-                    for (int c = 0; c < ocols; c += 32) {
-                        float o[32];
+                l = l * scale0 + ml.y * scale1;
+                m = t;
+#pragma unroll 1
+                for (int n = seg.n0 + 1; n < n1 && !both; n += 2) both = seg.see[0](n);
+            }
+            if (poison[w] || (!two && poison[1])) {
+                if (live) redo_rows<T>(x, seg, w, quarter);
+#pragma unroll 1
+                for (int k = 0; k < 2 && ok; ++k) {             // all have read the note; all see it taken back
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&met[w]);
+                    ok = wait(&met[w], meets++);
+                    if (k == 0) {
+                        poison[w] = 0;
+                        if (!two) poison[1] = 0;
+                    }
+                }
+                if (!ok) break;
+            } else if (live) {
+                const int h = seg.g * x.group + head, part_row = (two ? w : 0) * kTileQ + r;
+                float inv = scale0;
+                if (seg.whole) {
+                    if (a.sink && valid) l += ex2(a.sink[h] * kLog2e - m);
+                    const float f = valid && row >= 0 ? 1.f / l : 0.f;
+                    inv *= f;
+                    scale1 *= f;
+                    if (a.lse && valid) a.lse[(size_t)(it.token + token) * a.H + h] = m + log2f(l);
+                } else if (valid) {
+                    x.pl.ml[(size_t)seg.slot * x.pl.stride + part_row] = make_float2(m, l);
+                }
+                float4* parts = x.pl.o + (size_t)seg.slot * (p.E / 4) * x.pl.stride + part_row;
+#pragma unroll 1
+                for (int c = 0; c < ocols && (any || both); c += 32) {
+                    float o[32];
+                    if (any) {
                         tmem_ld_32x32(to + c, o);
-                        if (!valid) continue;
-                        if (wk.whole) {
 #pragma unroll
-                            for (int j = 0; j < 32; j += 8)
-                                if (c + j < p.E) {          // E is a multiple of 8
-                                    uint4 v;
-                                    v.x = pack2<T>(o[j] * inv, o[j + 1] * inv);
-                                    v.y = pack2<T>(o[j + 2] * inv, o[j + 3] * inv);
-                                    v.z = pack2<T>(o[j + 4] * inv, o[j + 5] * inv);
-                                    v.w = pack2<T>(o[j + 6] * inv, o[j + 7] * inv);
-                                    *reinterpret_cast<uint4*>(out + c + j) = v;
-                                }
-                        } else {
+                        for (int j = 0; j < 32; ++j) o[j] *= inv;
+                    } else {
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4)
-                                if (c + j < p.E) parts[(size_t)((c + j) / 4) * x.pl.stride] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        for (int j = 0; j < 32; ++j) o[j] = 0.f;
+                    }
+                    if (both) {
+                        float e[32];
+                        tmem_ld_32x32(to + 128 + c, e);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = fmaf(e[j], scale1, o[j]);
+                    }
+                    if (seg.whole) {
+                        // turned around in shared memory, so that four lanes write 64 bytes of a row
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            turn[lane * 4 + (j ^ ((lane >> 1) & 3))] = make_uint4(pack2<T>(o[8 * j], o[8 * j + 1]), pack2<T>(o[8 * j + 2], o[8 * j + 3]), pack2<T>(o[8 * j + 4], o[8 * j + 5]),
+                                                                                  pack2<T>(o[8 * j + 6], o[8 * j + 7]));
+                        __syncwarp();
+#pragma unroll 1
+                        for (int k = 0; k < 4; ++k) {
+                            const int from = 8 * k + (lane >> 2), j = lane & 3, u = quarter * 32 + from, t = u / x.group;
+                            const uint4 v = turn[from * 4 + (j ^ ((from >> 1) & 3))];
+                            if (u < x.tq * x.group && tile0 + t < it.count && c + 8 * j < p.E)
+                                *reinterpret_cast<uint4*>((T*)a.out + ((size_t)(it.token + tile0 + t) * a.H + seg.g * x.group + u - t * x.group) * p.E + c + 8 * j) = v;
                         }
+                        __syncwarp();
+                    } else if (valid) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            if (c + j < p.E) parts[(size_t)((c + j) / 4) * x.pl.stride] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                     }
                 }
             }
+            if (!two) {                  // the second group may go on
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&taken);
+                ++joins;
+            }
+            release(i);
         }
     }
     tc_fence_before();
@@ -430,14 +619,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
 
 // Joins the parts of items that several CTAs had, in their order.  Block b has the item that the boundary between CTAs b and b + 1 cuts, unless an earlier boundary cuts it too.
 template <class T>
-__global__ void __launch_bounds__(256) merge_kernel(const AttendArgs a, const Plan pl, int group, int tq) {
+__global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan pl, int group, int tq) {
     rcu_kernel_entry();
     const View& p = a.p;
     const int W = pl.head[0], C = pl.head[1], b = blockIdx.x;
     if (b + 1 >= C) return;
     const long long total = (long long)W * p.G;
     const int begin = first_tile(total, b, C), cut = first_tile(total, b + 1, C);
-    Walk wk(pl, b + 1, p.G);             // the item at the boundary
+    Walk wk(pl, b + 1, p.G, pl.items);             // the item at the boundary
     const int start = wk.g * W + pl.prefix[wk.i], stop = wk.g * W + pl.prefix[wk.i + 1];
     if (start == cut || start < begin) return;
     int parts = 1;                       // CTAs b .. b + parts - 1
@@ -504,9 +693,10 @@ template <class T> rcu_status launch(rcu_device* dev, const AttendArgs& a, int d
     TcArgs x{a, {}, a.H / p.G, kTileQ / (a.H / p.G), 0, (p.D + 63) / 64, (p.E + 63) / 64, 0};
     plan_of(dev, p, a.H, (char*)scratch, &x.pl);
     x.stage_bytes = (x.nb > x.eb ? x.nb : x.eb) * kBlock;
-    const int room = dev->smem_optin - 2048 - 2 * x.nb * kBlock;          // 1 KB to align, 1 KB of static shared memory
+    constexpr int kTurn = 8 * 2048;
+    const int room = dev->smem_optin - 3072 - kTurn - 2 * x.nb * kBlock;          // 1 KB to align, 2 KB of static shared memory
     x.stages = room / x.stage_bytes < kMostStages ? room / x.stage_bytes : kMostStages;
-    const size_t smem = 1024 + (size_t)2 * x.nb * kBlock + (size_t)x.stages * x.stage_bytes;
+    const size_t smem = 1024 + (size_t)2 * x.nb * kBlock + (size_t)x.stages * x.stage_bytes + kTurn;
     CUtensorMap qm, km, vm;
     if (!map_queries(&qm, dt, p, a.q, x.group, x.tq) || !map_pages(&km, dt, p, p.keys, p.D) || !map_pages(&vm, dt, p, p.values, p.E))
         return rcu_fail(dev, RCU_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (%d tokens, %d heads, %d pages)", p.T, a.H, p.pages);

@@ -100,7 +100,7 @@ struct MassArgs {
 };
 
 template <class T>
-__global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, MassArgs x) {
+__global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ MassArgs x) {
     extern __shared__ unsigned char smem_dyn[];
     const AttendArgs& a = x.a;
     const View& p = a.p;
@@ -150,13 +150,13 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
     tc_fence_after();
     rcu_kernel_entry_wait_only();        // nothing before this touches global memory
     const uint32_t tmem = tmem_slot;
-    x.pl.items = x.pl.head[2];
+    const int items = x.pl.head[2];
 
     if (warp == 0) {
         const int rows_box = min(p.R, kTileK), boxes = kTileK / rows_box, box = lane % boxes, col = lane / boxes;
         int item = 0, fills = 0;
         bool ok = true;
-        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next(), ++item) {
+        for (Walk wk(x.pl, blockIdx.x, p.G, items); wk.more() && ok; wk.next(), ++item) {
             const Seq q = seq_of(p, wk.it.s);
             const int j0 = wk.it.token * kTileK, b = item & 1;
             const int page = j0 + box * rows_box < q.L ? page_of(p, wk.it.s, j0 + box * rows_box) : -1;
@@ -204,10 +204,10 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
         const int ksteps = (p.D + 15) / 16;
         const uint64_t kd = umma_desc_sw128(ks), qd = umma_desc_sw128(ring);
         const bool leader = elect_one();
-        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait_spin(bar, phase & 1, &abort_flag, p.status)); };
+        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, &abort_flag, p.status)); };
         bool ok = true;
         int item = 0, at = 0;                    // at: query tiles so far
-        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next(), ++item) {
+        for (Walk wk(x.pl, blockIdx.x, p.G, items); wk.more() && ok; wk.next(), ++item) {
             const int b = item & 1;
             ok = wait(&k_full[b], item / 2);
             for (int n = wk.n0; n < wk.n1 && ok; ++n, ++at) {
@@ -237,10 +237,10 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
     } else {
         const int w = warp < 6 ? 0 : 1, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait_spin(bar, phase & 1, &abort_flag, p.status)); };
+        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, &abort_flag, p.status)); };
         bool ok = true;
         int item = 0, at = 0;
-        for (Walk wk(x.pl, blockIdx.x, p.G); wk.more() && ok; wk.next(), ++item) {
+        for (Walk wk(x.pl, blockIdx.x, p.G, items); wk.more() && ok; wk.next(), ++item) {
             const Seq q = seq_of(p, wk.it.s);
             const int j0 = wk.it.token * kTileK, j = j0 + r;
             float sum = 0.f;
@@ -253,40 +253,38 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
                 const int t0 = (wk.it.count + n) * x.tq, r0 = q.old() + t0, r1 = r0 + x.tq - 1;
                 // every query sees every row of the tile
                 const bool whole = t0 + x.tq <= q.n && j0 + kTileK - 1 <= r0 && (a.window == 0 || j0 > r1 - a.window || j0 + kTileK <= a.first);
-                float add[4] = {0.f, 0.f, 0.f, 0.f};
+                float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    float z[32];
+                    tmem_ld_32x32(tmem + 128 * t + 32 * q4 + lanes, z);
+                    const float4* ls = reinterpret_cast<const float4*>(&lse[s][32 * q4]);
+                    if (!whole) {            // a weight of 0 for what is not seen
+                        const int4* rs = reinterpret_cast<const int4*>(&rows[s][32 * q4]);
+                        auto hide = [&](float& score, int row) {
+                            if (j > row || (a.window > 0 && j <= row - a.window && j >= a.first)) score = -INFINITY;
+                        };
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float z[64];
-                    tmem_ld_32x64(tmem + 128 * t + 64 * half + lanes, z);
-                    const float4* ls = reinterpret_cast<const float4*>(&lse[s][64 * half]);
-                    const int4* rs = reinterpret_cast<const int4*>(&rows[s][64 * half]);
-                    if (whole) {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            const float4 v = ls[c];
-                            add[0] += ex2(fmaf(z[4 * c], a.c, -v.x));
-                            add[1] += ex2(fmaf(z[4 * c + 1], a.c, -v.y));
-                            add[2] += ex2(fmaf(z[4 * c + 2], a.c, -v.z));
-                            add[3] += ex2(fmaf(z[4 * c + 3], a.c, -v.w));
-                        }
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) {
-                            const float4 v = ls[c];
+                        for (int c = 0; c < 8; ++c) {
                             const int4 at4 = rs[c];
-                            auto weight = [&](float score, float l, int row) {
-                                const bool in = j <= row && (a.window == 0 || j > row - a.window || j < a.first);
-                                return in ? ex2(fmaf(score, a.c, -l)) : 0.f;
-                            };
-                            add[0] += weight(z[4 * c], v.x, at4.x);
-                            add[1] += weight(z[4 * c + 1], v.y, at4.y);
-                            add[2] += weight(z[4 * c + 2], v.z, at4.z);
-                            add[3] += weight(z[4 * c + 3], v.w, at4.w);
+                            hide(z[4 * c], at4.x);
+                            hide(z[4 * c + 1], at4.y);
+                            hide(z[4 * c + 2], at4.z);
+                            hide(z[4 * c + 3], at4.w);
                         }
                     }
+                    const float2 c2 = make_float2(a.c, a.c);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float4 v = ls[c];
+                        const float2 x0 = fma2(make_float2(z[4 * c], z[4 * c + 1]), c2, make_float2(-v.x, -v.y)), x1 = fma2(make_float2(z[4 * c + 2], z[4 * c + 3]), c2, make_float2(-v.z, -v.w));
+                        add[0] = add2(add[0], make_float2(ex2(x0.x), ex2(x0.y)));
+                        add[1] = add2(add[1], make_float2(ex2(x1.x), ex2(x1.y)));
+                    }
                 }
-                sum += (add[0] + add[1]) + (add[2] + add[3]);
                 tc_fence_before();
+                const float2 both = add2(add[0], add[1]);
+                sum += both.x + both.y;
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&s_empty[t]);
@@ -321,14 +319,13 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
 }
 
 // Adds the parts of tiles that several CTAs had, in their order (as merge_kernel).
-__global__ void __launch_bounds__(kTileK) mass_merge_kernel(const View p, Plan pl) {
+__global__ void __launch_bounds__(kTileK) mass_merge_kernel(const __grid_constant__ View p, const __grid_constant__ Plan pl) {
     rcu_kernel_entry();
     const int W = pl.head[0], C = pl.head[1], b = blockIdx.x;
-    pl.items = pl.head[2];
     if (b + 1 >= C) return;
     const long long total = (long long)W * p.G;
     const int begin = first_tile(total, b, C), cut = first_tile(total, b + 1, C);
-    Walk wk(pl, b + 1, p.G);
+    Walk wk(pl, b + 1, p.G, pl.head[2]);
     const int start = wk.g * W + pl.prefix[wk.i], stop = wk.g * W + pl.prefix[wk.i + 1];
     if (start == cut || start < begin) return;
     const float* parts = reinterpret_cast<const float*>(pl.ml);

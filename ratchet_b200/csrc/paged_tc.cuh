@@ -16,6 +16,129 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+template <class T> __device__ __forceinline__ uint32_t pack2(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two f32 operations of one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 32 lanes x 32 columns of tensor memory -> 32 registers per thread, not waited for (tmem_ld_wait)
+__device__ __forceinline__ void tmem_ld_32x32_start(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// 2^x for two numbers on the FMA pipe, which the exponential unit (four results a cycle and quarter of an SM) leaves idle.  x = n + f with n whole and
+// |f| <= 1/2 (n appears in the low bits of x + 1.5 2^23); 2^f by a polynomial of degree 4 fitted to the least relative error (2.6e-6), times 2^n.
+// x up to 127; below -126 the result is 0; NaN stays NaN.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+    constexpr float kMagic = 12582912.f + 127.f;
+    x = make_float2(max_nan(x.x, -127.f), max_nan(x.y, -127.f));
+    const float2 t = add2(x, make_float2(kMagic, kMagic));
+    const float2 f = fma2(add2(t, make_float2(-kMagic, -kMagic)), make_float2(-1.f, -1.f), x);
+    float2 y = fma2(make_float2(0.009570101276040077f, 0.009570101276040077f), f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    y = fma2(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    return mul2(y, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
+}
+// 16 registers per thread -> 32 lanes x 16 columns of tensor memory, not waited for
+__device__ __forceinline__ void tmem_st_32x16_start(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A place in a ring of `n` stages, and the parity of its barriers' phase
+struct RingAt {
+    int n, s, phase;
+    __device__ __forceinline__ void go(int k) {
+        s += k;
+        if (s >= n) {
+            s -= n;
+            phase ^= 1;
+        }
+    }
+};
+
+// A bounded wait whose common end is one instruction; the rest stays out of line, because these kernels are as long as the instruction cache
+static __device__ __noinline__ bool wait_on(uint64_t* bar, int phase, volatile int* abort_flag, int* status) { return gemvq8::mbar_wait(bar, phase, abort_flag, status); }
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, int phase, volatile int* abort_flag, int* status) {
+    bool ok = gemvq8::mbar_try_wait(bar, phase & 1);
+    if (!__all_sync(0xffffffffu, ok)) ok = __all_sync(0xffffffffu, ok || wait_on(bar, phase & 1, abort_flag, status));
+    return ok;
+}
+// lets a copy land before the memory is somebody else's; bounded
+static __device__ __noinline__ void land(uint64_t* bar, int phase) {
+#pragma unroll 1
+    for (int k = 0; k < (1 << 16) && !gemvq8::mbar_test_wait(bar, phase & 1); ++k) {}
+}
+
+// Page ids of a sequence, 32 consecutive ones in the warp's lanes
+struct PageIds {
+    int from = -64, id = 0;
+    // id of page i (of the sequence's table) for this lane; `first` .. `first` + 31 covers all lanes' pages, `pages` of them exist
+    __device__ __forceinline__ int of(const View& p, int s, int first, int i, int last_first, int pages) {
+        if (first < from || last_first >= from + 32) {
+            from = first;
+            const int at = first + (int)(threadIdx.x & 31);
+            id = at < pages ? p.table[(size_t)s * p.MP + at] : 0;
+            if (at < pages && (unsigned)id >= (unsigned)p.pages) {
+                report_bad(p.status);
+                id = 0;
+            }
+        }
+        return __shfl_sync(0xffffffffu, id, i - from);
+    }
+};
+
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int u, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_u32(bar))
