@@ -39,10 +39,11 @@ struct Plan {
     int items;                 // upper bound: T / tokens + S
     int tokens;                // of an item
     int ctas, least;           // CTAs at most; tiles that a CTA takes at least
-    int rows, stride;          // rows of a tile (tokens / 2 * group), of a part in scratch
+    int extra;                 // see Walk
+    int stride;                // rows of a part in scratch
     // scratch
-    int* head;                 // [0] tiles of a kv head, [1] CTAs at work
-    int* prefix;               // [items + 1]: tiles of a kv head's items before each
+    int* head;                 // [0] length of a kv head, [1] CTAs at work
+    int* prefix;               // [items + 1]: where each item of a kv head begins
     Item* item;                // [items]
     float2* ml;                // [2 * ctas, stride]: a part's maximum and sum, per row
     float4* o;                 // [2 * ctas, E / 4, stride]: its weighted sum of values
@@ -67,53 +68,87 @@ __device__ __forceinline__ Span span_of(int window, int first, int r0, int r1) {
 // The tiles that CTA b of C takes of `total`
 __device__ __forceinline__ int first_tile(long long total, int b, int C) { return (int)(total * b / C); }
 
-// A CTA's walk over its run: item by item
+// The item at place y of a kv head's row
+__device__ __forceinline__ int item_at(const Plan& pl, int items, int y) {
+    int lo = 0, hi = items - 1;                  // the last item that begins there or before
+#pragma unroll 1
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (pl.prefix[mid] <= y) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// A CTA's walk over its run: item by item.  An item's place in the row of all is as long as its tiles and `extra` more, which stand for what beginning
+// and ending it costs: nothing is done in these.
 struct Walk {
     const Plan& pl;
-    int items, W, at, end, begin;     // items and tiles of a kv head; run
+    int items, W, at, end;     // items, length of a kv head; run
     int g, i;                  // kv head and item at `at`
     Item it;
-    int n0, n1, whole;         // tiles [n0, n1) of the item; whether these are all of them
+    int n0, n1, whole;         // tiles [n0, n1) of the item, not empty; whether these are all of them
     __device__ __forceinline__ Walk(const Plan& plan, int b, int G, int count) : pl(plan), items(count) {
         W = plan.head[0];
         const int C = plan.head[1];
         const long long total = (long long)W * G;
-        at = begin = b < C ? first_tile(total, b, C) : 0;
+        at = b < C ? first_tile(total, b, C) : 0;
         end = b < C ? first_tile(total, b + 1, C) : 0;
-        if (at < end) find();
+        if (at >= end) return;
+        find();
+        if (n0 >= n1) next();
     }
+    // the item at place `at`, and what of it lies before `end`
     __device__ __forceinline__ void find() {
         g = at / W;
-        const int y = at - g * W;
-        int lo = 0, hi = items - 1;                  // the last item with prefix <= y
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (pl.prefix[mid] <= y) lo = mid;
-            else hi = mid - 1;
-        }
-        i = lo;
+        i = item_at(pl, items, at - g * W);
         load();
     }
     __device__ __forceinline__ void load() {
         it = pl.item[i];
-        const int p0 = g * W + pl.prefix[i], p1 = g * W + pl.prefix[i + 1];
-        n0 = at - p0;
+        const int p0 = g * W + pl.prefix[i] + pl.extra, p1 = g * W + pl.prefix[i + 1];
+        n0 = max(0, at - p0);
         n1 = min(end, p1) - p0;
         whole = n0 == 0 && p0 + n1 == p1;
     }
     __device__ __forceinline__ bool more() const { return at < end; }
-    __device__ __forceinline__ int slot(int b) const { return 2 * b + (at != begin); }
+    // a CTA has one part that goes on with an item at most, and one that begins an item and does not end it
+    __device__ __forceinline__ int slot(int b) const { return 2 * b + (n0 == 0); }
     __device__ __forceinline__ void next() {
-        at += n1 - n0;
-        if (at >= end) return;
-        if (at >= (g + 1) * W) {
-            ++g;
-            i = -1;
-        }
-        do ++i;
-        while (pl.prefix[i + 1] == pl.prefix[i]);       // ends: at < end <= W G, so a later item has tiles
-        load();
+        do {
+            at = g * W + pl.prefix[i + 1];
+            if (at >= end) return;
+            if (at >= (g + 1) * W) {
+                ++g;
+                i = -1;
+            }
+            do ++i;
+            while (pl.prefix[i + 1] == pl.prefix[i]);       // ends: at < end <= W G, so a later item has a place
+            load();
+        } while (n0 >= n1);
     }
+};
+
+// The parts that have to be joined at the boundary between CTAs b and b + 1: `count` of them, the first in slot 2 b + 1, the others in slots
+// 2 (b + 1), 2 (b + 2), ..; none where the boundary cuts no item's tiles, or an earlier one has cut the same item
+struct Join {
+    int count;
+    int g;
+    Item it;
+    __device__ __forceinline__ Join(const Plan& pl, int b, int G, int items) : count(0) {
+        const int W = pl.head[0], C = pl.head[1];
+        if (b + 1 >= C) return;
+        const long long total = (long long)W * G;
+        const int before = first_tile(total, b, C), cut = first_tile(total, b + 1, C);
+        if (cut >= total) return;
+        g = cut / W;
+        const int i = item_at(pl, items, cut - g * W), p0 = g * W + pl.prefix[i] + pl.extra, p1 = g * W + pl.prefix[i + 1];
+        if (cut <= p0 || before > p0) return;
+        it = pl.item[i];
+        count = 1;
+        while (b + count < C && first_tile(total, b + count, C) < p1) ++count;
+    }
+    __device__ __forceinline__ int slot(int b, int k) const { return k == 0 ? 2 * b + 1 : 2 * (b + k); }
 };
 #endif
 

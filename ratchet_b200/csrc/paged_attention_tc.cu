@@ -7,8 +7,9 @@
 //   warp 1              per tile n and query tile w: O_w += P_w V of tile n - 1, with P_w read from tensor memory, then S_w = Q_w K^T of tile n,
 //                       which takes P_w's place;
 //   warps 4-7, 8-11     softmax of query tile 0 / 1, a query per thread: scores from tensor
-//                       memory, mask, running maximum, weights back over the scores in two halves.  The maximum that weights are taken against
-//                       only moves when a score exceeds it by more than 2^8, so that O_w is rescaled rarely.
+//                       memory, mask, running maximum, weights back over the scores, half a tile of rows at a time: the scores of one half are there
+//                       while the weights of the other are worked out.  The maximum that weights are taken against only moves when a score exceeds
+//                       it by more than 2^8, so that O_w is rescaled rarely.
 // An item of one query tile (generation) gives it to both groups, which take the tiles of rows in turns and join their sums at the end.
 // Weights enter the second product in the operands' type: half a step of theirs moves the sum by as much as the rounding of the output does.  Their
 // sum, the maximum and O are f32.
@@ -57,6 +58,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const View p, const Plan pl,
             if (at >= 0 && at < q.n) {
                 it = Item{lo, q.start + at, min(pl.tokens, q.n - at), q.old() + at};
                 w = span_of(window, first, it.row, min(it.row + it.count, q.L) - 1).count;
+                w += w > 0 ? pl.extra : 0;
             }
             pl.item[i] = it;
         }
@@ -144,8 +146,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
     const View& p = a.p;
     unsigned char* qs = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
     unsigned char* ring = qs + 2 * x.nb * kBlock;
-    // p_full: a half of the tile's rows each, so that the product with V begins while the second half's weights are worked out
-    __shared__ __align__(8) uint64_t q_full, q_empty, full[kMostStages], empty[kMostStages], s_full[2], p_full[2][2], o_full[2], met[2], joined, taken, drained,
+    // [query tile][half of a tile of rows]
+    __shared__ __align__(8) uint64_t q_full, q_empty, full[kMostStages], empty[kMostStages], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], met[2], joined, taken, drained,
         seg_full[kSegments], seg_empty[kSegments];
     __shared__ Segment segments[kSegments];
     __shared__ float2 other[kTileQ];                  // maximum and sum that the second group hands to the first
@@ -171,9 +173,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         }
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
+            mbar_init(&s_full[i][0], 1);
+            mbar_init(&s_full[i][1], 1);
             mbar_init(&p_full[i][0], 4);
             mbar_init(&p_full[i][1], 4);
+            mbar_init(&pv_done[i], 1);
             mbar_init(&o_full[i], 1);
             mbar_init(&met[i], 4);
             poison[i] = 0;
@@ -259,12 +263,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
             }
             __syncwarp();
             PageIds ids;
-            const int L = seg.L, have = min(p.MP, (L + p.R - 1) >> p.shift);
+            const int L = seg.L, have = min(p.MP, (L + p.R - 1) >> p.shift), s_id = seg.it.s, g = seg.g, n1 = seg.n1;
+            const Span sp = seg.sp;
 #pragma unroll 1
-            for (int n = seg.n0; n < seg.n1 && ok; ++n) {
-                const int j0 = seg.sp.tile(n) * kTileK, i0 = j0 >> p.shift, row0 = j0 & (p.R - 1);
+            for (int n = seg.n0; n < n1 && ok; ++n) {
+                const int j0 = sp.tile(n) * kTileK, i0 = j0 >> p.shift, row0 = j0 & (p.R - 1);
                 const bool in = j0 + box * rows_box < L;               // boxes behind the last row are left out
-                const int page = ids.of(p, seg.it.s, i0, i0 + box, i0 + boxes - 1, have);
+                const int page = ids.of(p, s_id, i0, i0 + box, i0 + boxes - 1, have);
                 const int pages = min(boxes, (L - j0 + rows_box - 1) / rows_box);
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv) {
@@ -273,7 +278,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                     if (lane == 0) mbar_expect_tx(&full[at.s], pages * (kv ? x.eb : x.nb) * rows_box * 128);
                     __syncwarp();
                     if ((kv ? mine_v : mine_k) && in)
-                        tma_load_4d(ring + (size_t)at.s * x.stage_bytes + col * kBlock + box * rows_box * 128, kv ? &vmap : &kmap, col * 64, row0, seg.g, page, &full[at.s]);
+                        tma_load_4d(ring + (size_t)at.s * x.stage_bytes + col * kBlock + box * rows_box * 128, kv ? &vmap : &kmap, col * 64, row0, g, page, &full[at.s]);
                     at.go(1);
                     ++fills;
                 }
@@ -287,88 +292,92 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
             land(&q_full, i);
         }
     } else if (warp == 1) {
-        // the whole warp keeps step, one elected lane issues
-        constexpr bool bf16 = !std::is_same<T, __half>::value;
-        const uint32_t idesc_s = umma_idesc_f16(kTileQ, kTileK, bf16);
-        const uint32_t idesc_o = umma_idesc_f16(kTileQ, (p.E + 15) & ~15, bf16) | (1u << 16);     // V is stored with its columns contiguous
-        const int ksteps = (p.D + 15) / 16;
-        const uint64_t qd = umma_desc_sw128(qs), kd = umma_desc_sw128(ring), vd = umma_desc_sw128_mn(ring, kBlock);
-        const bool leader = elect_one();
-        bool ok = true;
-        int weights0 = 0, weights1 = 0;                // hand-overs of P_w so far
-        RingAt kat{x.stages, 0, 0}, vat{x.stages, 1, 0};
+        // one lane: what it does between two products, tensor memory waits for
+        if (elect_one()) {
+            constexpr bool bf16 = !std::is_same<T, __half>::value;
+            const uint32_t idesc_s = umma_idesc_f16(kTileQ, kTileK / 2, bf16);
+            const uint32_t idesc_o = umma_idesc_f16(kTileQ, (p.E + 15) & ~15, bf16) | (1u << 16);     // V is stored with its columns contiguous
+            const int ksteps = (p.D + 15) / 16, stage16 = x.stage_bytes >> 4;
+            const uint64_t qd = umma_desc_sw128(qs), kd = umma_desc_sw128(ring), vd = umma_desc_sw128_mn(ring, kBlock);
+            auto wait1 = [&](uint64_t* bar, int phase) { return gemvq8::mbar_try_wait(bar, phase & 1) || wait_on(bar, phase & 1, &abort_flag, p.status); };
+            bool ok = true;
+            int weights0 = 0, weights1 = 0;                // hand-overs of P_w so far
+            RingAt kat{x.stages, 0, 0}, vat{x.stages, 1, 0};
 #pragma unroll 1
-        for (int i = 0;; ++i) {
-            const Segment& seg = take(i, ok);
-            if (!ok || !seg.more) break;
-            const int n0 = seg.n0, n1 = seg.n1;
-            const bool two = seg.two;
-            bool any0 = false, any1 = false;
-            ok = wait(&q_full, i);
+            for (int i = 0;; ++i) {
+                ok = wait1(&seg_full[i % kSegments], i / kSegments);
+                const Segment seg = segments[i % kSegments];
+                if (!ok || !seg.more) break;
+                mbar_arrive(&seg_empty[i % kSegments]);
+                bool any0 = false, any1 = false, v0 = false, v1 = false;
+                ok = wait1(&q_full, i);
+                // Half a tile of rows at a time, two halves in flight: while the weights of one are worked out, the scores of the other are there.
+                // At place n the products with V of tile n - 1, and the scores of tile n, half by half, in the same columns.
 #pragma unroll 1
-            for (int n = n0; n <= n1 && ok; ++n) {
-                const bool last = n == n1;
-                const uint64_t kb = kd + (uint64_t)(kat.s * (x.stage_bytes >> 4)), vb = vd + (uint64_t)(vat.s * (x.stage_bytes >> 4));
-                auto scores = [&](auto w) {
-                    if (last || !seg.has(w, n)) return;
-                    tc_fence_after();
-                    if (leader) {
-                        const uint64_t qa = qd + (uint64_t)((two ? w() : 0) * x.nb * (kBlock >> 4));
+                for (int n = seg.n0; n <= seg.n1 && ok; ++n) {
+                    const bool first = n == seg.n0, last = n == seg.n1;
+                    const uint64_t kb = kd + (uint64_t)(kat.s * stage16), vb = vd + (uint64_t)(vat.s * stage16);
+                    const bool s0 = !last && seg.has(0, n), s1 = !last && seg.has(1, n);
+                    auto scores = [&](auto w, int half) {
+                        tc_fence_after();
+                        const uint64_t qa = qd + (uint64_t)((seg.two ? w() : 0) * x.nb * (kBlock >> 4)), ka = kb + 512 * half;
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            if (k < ksteps) umma_f16(tmem + 128 * w, qa + (k >> 2) * (kBlock >> 4) + 2 * (k & 3), kb + (k >> 2) * (kBlock >> 4) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
-                        umma_commit(&s_full[w]);
-                    }
-                    __syncwarp();
-                };
-                auto values = [&](auto w, int& weights, bool& any) {
-                    if (n == n0 || !seg.has(w, n - 1)) return;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (ok) ok = wait(&p_full[w][half], weights);
+                            if (k < ksteps)
+                                umma_f16(tmem + 128 * w + 64 * half, qa + (k >> 2) * (kBlock >> 4) + 2 * (k & 3), ka + (k >> 2) * (kBlock >> 4) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
+                        umma_commit(&s_full[w][half]);
+                    };
+                    auto values = [&](auto w, int half, int weights, bool more) {
+                        ok = wait1(&p_full[w][half], weights);
+                        if (!ok) return;
                         tc_fence_after();
-                        if (ok && leader) {
 #pragma unroll
-                            for (int k = 4 * half; k < 4 * half + 4; ++k)      // 16 rows are two 1024-byte groups of V, eight columns of P
-                                umma_f16_ta(tmem + 256 + 128 * w, tmem + 128 * w + 8 * k, vb + 128 * k, idesc_o, k > 0 || any ? 1u : 0u);
+                        for (int k = 0; k < 4; ++k)      // 16 rows are two 1024-byte groups of V, eight columns of P
+                            umma_f16_ta(tmem + 256 + 128 * w, tmem + 128 * w + 64 * half + 8 * k, vb + 512 * half + 128 * k, idesc_o, k > 0 || more ? 1u : 0u);
+                        umma_commit(&pv_done[w]);
+                    };
+                    using W0 = std::integral_constant<int, 0>;
+                    using W1 = std::integral_constant<int, 1>;
+                    if (!last) ok = wait1(&full[kat.s], kat.phase);
+                    if (!ok) break;
+                    // in turns, the two groups' tiles are different ones: the scores of one need not wait for the weights of the other
+                    if (!seg.two) {
+#pragma unroll 1
+                        for (int half = 0; half < 2; ++half) {
+                            if (s0) scores(W0{}, half);
+                            if (s1) scores(W1{}, half);
                         }
-                        __syncwarp();
                     }
-                    ++weights;
-                    any = true;
-                };
-                using W0 = std::integral_constant<int, 0>;
-                using W1 = std::integral_constant<int, 1>;
-                if (!last) ok = wait(&full[kat.s], kat.phase);
-                if (!ok) break;
-                // in turns, the two groups' tiles are different ones: the scores of one need not wait for the weights of the other
-                if (!two) {
-                    scores(W0{});
-                    scores(W1{});
-                }
-                if (n > n0) ok = wait(&full[vat.s], vat.phase);
-                if (ok) values(W0{}, weights0, any0);
-                if (ok && two) scores(W0{});
-                if (ok) values(W1{}, weights1, any1);
-                if (ok && two) scores(W1{});
-                if (!ok) break;
-                if (leader) {
+                    if (!first) ok = wait1(&full[vat.s], vat.phase);
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        if (ok && v0) values(W0{}, half, weights0, any0 || half);
+                        if (ok && seg.two && s0) scores(W0{}, half);
+                        if (ok && v1) values(W1{}, half, weights1, any1 || half);
+                        if (ok && seg.two && s1) scores(W1{}, half);
+                    }
+                    if (!ok) break;
+                    weights0 += v0;
+                    weights1 += v1;
+                    any0 |= v0;
+                    any1 |= v1;
+                    v0 = s0;
+                    v1 = s1;
                     if (!last) umma_commit(&empty[kat.s]);
-                    if (n == n1 - 1) umma_commit(&q_empty);
-                    if (n > n0) umma_commit(&empty[vat.s]);
+                    if (n == seg.n1 - 1) umma_commit(&q_empty);
+                    if (!first) umma_commit(&empty[vat.s]);
                     if (last && any0) umma_commit(&o_full[0]);
                     if (last && any1) umma_commit(&o_full[1]);
+                    if (!last) kat.go(2);
+                    if (!first) vat.go(2);
                 }
-                __syncwarp();
-                if (!last) kat.go(2);
-                if (n > n0) vat.go(2);
+                if (!ok) break;
             }
-            if (!ok) break;
-            release(i);
-        }
-        if (!ok && leader) {            // given up: let the products in flight end before tensor memory is freed
-            umma_commit(&drained);
-            for (int k = 0; k < 16; ++k) land(&drained, 0);
+            if (!ok) {            // given up: let the products in flight end before tensor memory is freed
+                umma_commit(&drained);
+#pragma unroll 1
+                for (int k = 0; k < 16; ++k) land(&drained, 0);
+            }
         }
         __syncwarp();
     } else if (warp >= 4) {
@@ -378,16 +387,26 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, ts = tmem + 128 * w + lanes, to = tmem + 256 + 128 * w + lanes;
         const int ocols = (p.E + 31) & ~31;
         uint4* turn = reinterpret_cast<uint4*>(ring + (size_t)x.stages * x.stage_bytes) + (warp - 4) * 128;      // 32 rows of 64 bytes, the warp's own
-        int scores = 0, outs = 0, meets = 0, joins = 0;
+        int tiles = 0, products = 0, outs = 0, meets = 0, joins = 0;      // tiles and halves of them so far
         RingAt vat{x.stages, 1, 0};
         bool ok = true;
+        // places of the output that this lane writes once rows are turned around: token of the tile, elements from its first row on
+        int turn_token[4], turn_at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int u = quarter * 32 + 8 * k + (lane >> 2);
+            turn_token[k] = u < x.tq * x.group ? u / x.group : 1 << 20;
+            turn_at[k] = (u / x.group * a.H + u % x.group) * p.E + 8 * (lane & 3);
+        }
 #pragma unroll 1
         for (int i = 0;; ++i) {
             const Segment& seg = take(i, ok);
             if (!ok || !seg.more) break;
             const bool two = seg.two;
             const Item it = seg.it;
-            const int tile0 = two ? w * x.tq : 0, token = tile0 + own, L = seg.L, n1 = seg.n1;
+            const Sight see = seg.see[w];            // copies: what is in shared memory is read again behind every wait
+            const Span sp = seg.sp;
+            const int tile0 = two ? w * x.tq : 0, token = tile0 + own, L = seg.L, n0 = seg.n0, n1 = seg.n1;
             const bool valid = r < x.tq * x.group && token < it.count;
             const int row = it.row + token;
             const bool live = __any_sync(0xffffffffu, valid);               // warps without a query only keep step
@@ -397,9 +416,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
             float m = valid ? -INFINITY : INFINITY, l = 0.f;                // a row of no query never moves the maximum
             bool any = false;
 #pragma unroll 1
-            for (int n = seg.n0; n < n1; ++n, vat.go(2)) {
-                if (!seg.has(w, n)) continue;
-                const int j0 = seg.sp.tile(n) * kTileK;
+            for (int n = n0; n < n1; ++n, vat.go(2)) {
+                if (!see(n) || (!two && ((n - n0) & 1) != w)) continue;
+                const int j0 = sp.tile(n) * kTileK;
                 // a tile that is not whole to all queries: rows behind the last one become zero, values that are not finite are noted
                 if (j0 + kTileK - 1 > t0 || (a.window > 0 && j0 <= t1 - a.window && j0 + kTileK > a.first)) {
                     ok = wait(&full[vat.s], vat.phase);
@@ -417,87 +436,70 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                     if (bad) poison[w] = 1;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                ok = wait(&s_full[w], scores++);
-                if (!ok) break;
-                tc_fence_after();
-                auto hand_over = [&](int half) {
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    ok = wait(&s_full[w][half], tiles);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (live) {
+                        const int j1 = j0 + 64 * half;
+                        float s[64];
+                        tmem_ld_32x64(ts + 64 * half, s);
+                        if (j1 + 63 > w0 || (a.window > 0 && j1 <= w1 - a.window && j1 + 64 > a.first)) {
+                            asm volatile("" ::: "memory");          // a branch, not 64 predicated selections in every tile
+                            const int hi = row - j1, lo = a.window > 0 ? hi - a.window : -1, head_end = a.first - j1;
+#pragma unroll
+                            for (int j = 0; j < 64; ++j)
+                                if (j > hi || (j <= lo && j >= head_end)) s[j] = -INFINITY;
+                        }
+                        float top4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                        for (int j = 4; j < 60; j += 8)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], s[j + e], s[j + 4 + e]);
+                        const float top = max3(max3(top4[0], top4[1], top4[2]), max3(top4[3], s[60], s[61]), fmaxf(s[62], s[63])) * a.c;      // c > 0
+                        const bool move = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
+                        const float next = move ? top : m;
+                        const float corr = move ? ex2(m - next) : 1.f;                    // 0 while no key has been seen
+                        m = next;
+                        const float z = m == -INFINITY ? 0.f : -m;
+                        // O may be rescaled behind the last product with V; the one before that was ahead of these scores
+                        if (any && __any_sync(0xffffffffu, move)) {
+                            ok = wait(&pv_done[w], products - 1);
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < ocols; c += 32) {
+                                float o[32];
+                                tmem_ld_32x32(to + c, o);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] *= corr;
+                                tmem_st_32x32(to + c, reinterpret_cast<const uint32_t*>(o));
+                            }
+                        }
+                        const float2 c2 = make_float2(a.c, a.c), z2 = make_float2(z, z);
+                        float2 l4[4] = {make_float2(l * corr, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                        uint32_t pw[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float2 t = fma2(make_float2(s[2 * j], s[2 * j + 1]), c2, z2);
+                            // every fourth pair on the FMA pipe, which takes that off the exponential unit
+                            const float2 u = (j & 3) == 3 ? ex2_fma(t) : make_float2(ex2(t.x), ex2(t.y));
+                            l4[j & 3] = add2(l4[j & 3], u);
+                            pw[j] = pack2<T>(u.x, u.y);
+                        }
+                        tmem_st_32x32(ts + 64 * half, pw);
+                        const float2 lb = add2(add2(l4[0], l4[1]), add2(l4[2], l4[3]));
+                        l = lb.x + lb.y;
+                    }
+                    any = true;
+                    ++products;
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&p_full[w][half]);
-                };
-                if (!live) {
-                    hand_over(0);
-                    hand_over(1);
-                    any = true;
-                    continue;
                 }
-                // 32 columns at a time, read twice (masked ones are written back the first time): tensor memory gives them in 70 cycles, and loops of a
-                // few kilobytes stay in the instruction cache
-                const bool masked = j0 + kTileK - 1 > w0 || (a.window > 0 && j0 <= w1 - a.window && j0 + kTileK > a.first);
-                float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float s[32];
-                    tmem_ld_32x32(ts + 32 * c, s);
-                    if (masked) {
-                        const int hi = row - j0 - 32 * c, lo = a.window > 0 ? hi - a.window : -1, head_end = a.first - j0 - 32 * c;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (j > hi || (j <= lo && j >= head_end)) s[j] = -INFINITY;
-                        tmem_st_32x32(ts + 32 * c, reinterpret_cast<const uint32_t*>(s));
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], s[j + e], s[j + 4 + e]);
-                }
-                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * a.c;      // c > 0
-                const bool move = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
-                const float next = move ? top : m;
-                const float corr = move ? ex2(m - next) : 1.f;                    // 0 while no key has been seen
-                m = next;
-                const float z = m == -INFINITY ? 0.f : -m;
-                // the scores came behind the product of the tile before with V: O may be rescaled
-                if (any && __any_sync(0xffffffffu, move)) {
-#pragma unroll 1
-                    for (int c = 0; c < ocols; c += 32) {
-                        float o[32];
-                        tmem_ld_32x32(to + c, o);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] *= corr;
-                        tmem_st_32x32(to + c, reinterpret_cast<const uint32_t*>(o));
-                    }
-                }
-                any = true;
-                const float2 c2 = make_float2(a.c, a.c), z2 = make_float2(z, z);
-                float2 l4[4] = {make_float2(l * corr, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                auto weigh = [&](const float (&s)[32], int c) {
-                    uint32_t pw[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float2 t = fma2(make_float2(s[2 * j], s[2 * j + 1]), c2, z2);
-                        // every fourth pair on the FMA pipe, which takes that off the exponential unit
-                        const float2 u = (j & 3) == 3 ? ex2_fma(t) : make_float2(ex2(t.x), ex2(t.y));
-                        l4[j & 3] = add2(l4[j & 3], u);
-                        pw[j] = pack2<T>(u.x, u.y);
-                    }
-                    tmem_st_32x16_start(ts + 16 * c, pw);          // over columns that have been read
-                };
-                float s0[32], s1[32];
-                tmem_ld_32x32_start(ts, s0);
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    tmem_ld_wait();
-                    tmem_ld_32x32_start(ts + 64 * half + 32, s1);
-                    weigh(s0, 2 * half);
-                    tmem_ld_wait();
-                    if (half == 0) tmem_ld_32x32_start(ts + 64, s0);
-                    weigh(s1, 2 * half + 1);
-                    tmem_st_wait();
-                    hand_over(half);
-                }
-                const float2 lb = add2(add2(l4[0], l4[1]), add2(l4[2], l4[3]));
-                l = lb.x + lb.y;
+                if (!ok) break;
+                ++tiles;
             }
             if (!ok) break;
             if (any) {
@@ -561,6 +563,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                 } else if (valid) {
                     x.pl.ml[(size_t)seg.slot * x.pl.stride + part_row] = make_float2(m, l);
                 }
+                T* out = (T*)a.out + ((size_t)(it.token + tile0) * a.H + seg.g * x.group) * p.E;
                 float4* parts = x.pl.o + (size_t)seg.slot * (p.E / 4) * x.pl.stride + part_row;
 #pragma unroll 1
                 for (int c = 0; c < ocols && (any || both); c += 32) {
@@ -586,12 +589,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                             turn[lane * 4 + (j ^ ((lane >> 1) & 3))] = make_uint4(pack2<T>(o[8 * j], o[8 * j + 1]), pack2<T>(o[8 * j + 2], o[8 * j + 3]), pack2<T>(o[8 * j + 4], o[8 * j + 5]),
                                                                                   pack2<T>(o[8 * j + 6], o[8 * j + 7]));
                         __syncwarp();
-#pragma unroll 1
+#pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const int from = 8 * k + (lane >> 2), j = lane & 3, u = quarter * 32 + from, t = u / x.group;
-                            const uint4 v = turn[from * 4 + (j ^ ((from >> 1) & 3))];
-                            if (u < x.tq * x.group && tile0 + t < it.count && c + 8 * j < p.E)
-                                *reinterpret_cast<uint4*>((T*)a.out + ((size_t)(it.token + tile0 + t) * a.H + seg.g * x.group + u - t * x.group) * p.E + c + 8 * j) = v;
+                            const int from = 8 * k + (lane >> 2);
+                            const uint4 v = turn[from * 4 + ((lane & 3) ^ ((from >> 1) & 3))];
+                            if (tile0 + turn_token[k] < it.count && c + 8 * (lane & 3) < p.E) *reinterpret_cast<uint4*>(out + turn_at[k] + c) = v;
                         }
                         __syncwarp();
                     } else if (valid) {
@@ -622,31 +624,23 @@ template <class T>
 __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan pl, int group, int tq) {
     rcu_kernel_entry();
     const View& p = a.p;
-    const int W = pl.head[0], C = pl.head[1], b = blockIdx.x;
-    if (b + 1 >= C) return;
-    const long long total = (long long)W * p.G;
-    const int begin = first_tile(total, b, C), cut = first_tile(total, b + 1, C);
-    Walk wk(pl, b + 1, p.G, pl.items);             // the item at the boundary
-    const int start = wk.g * W + pl.prefix[wk.i], stop = wk.g * W + pl.prefix[wk.i + 1];
-    if (start == cut || start < begin) return;
-    int parts = 1;                       // CTAs b .. b + parts - 1
-    while (b + parts < C && first_tile(total, b + parts, C) < stop) ++parts;
-    const int first_slot = 2 * b + (start != begin);
-    auto slot = [&](int i) { return i == 0 ? first_slot : 2 * (b + i); };
-    const int rows = wk.it.count * group, quads = p.E / 4;
+    const int b = blockIdx.x;
+    const Join jn(pl, b, p.G, pl.items);
+    if (jn.count == 0) return;
+    const int rows = jn.it.count * group, quads = p.E / 4;
     for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += gridDim.y * 256) {
-        const int u = i % rows, c = i / rows, token = u / group, h = wk.g * group + u % group;
+        const int u = i % rows, c = i / rows, token = u / group, h = jn.g * group + u % group;
         const int r = token / tq * kTileQ + u - token / tq * tq * group;
         float m = -INFINITY;
-        for (int k = 0; k < parts; ++k) m = fmaxf(m, pl.ml[(size_t)slot(k) * pl.stride + r].x);
+        for (int k = 0; k < jn.count; ++k) m = fmaxf(m, pl.ml[(size_t)jn.slot(b, k) * pl.stride + r].x);
         const float sk = a.sink ? a.sink[h] * kLog2e : -INFINITY, top = fmaxf(m, sk);
         float l = a.sink ? ex2(sk - top) : 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < parts; ++k) {
-            const float2 ml = pl.ml[(size_t)slot(k) * pl.stride + r];
+        for (int k = 0; k < jn.count; ++k) {
+            const float2 ml = pl.ml[(size_t)jn.slot(b, k) * pl.stride + r];
             if (ml.x == -INFINITY && ml.y == 0.f) continue;          // a part that sees nothing has no sum
             const float w = ex2(ml.x - top);
-            const float4 v = pl.o[((size_t)slot(k) * quads + c) * pl.stride + r];
+            const float4 v = pl.o[((size_t)jn.slot(b, k) * quads + c) * pl.stride + r];
             l = fmaf(ml.y, w, l);
             o.x = fmaf(v.x, w, o.x);
             o.y = fmaf(v.y, w, o.y);
@@ -654,7 +648,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Atte
             o.w = fmaf(v.w, w, o.w);
         }
         const float inv = 1.f / l;
-        const size_t at = (size_t)(wk.it.token + token) * a.H + h;
+        const size_t at = (size_t)(jn.it.token + token) * a.H + h;
         uint2 v;
         v.x = pack2<T>(o.x * inv, o.y * inv);
         v.y = pack2<T>(o.z * inv, o.w * inv);
@@ -671,7 +665,8 @@ uint64_t plan_of(const rcu_device* dev, const View& p, int H, char* mem, Plan* o
     pl.items = p.T / pl.tokens + p.S;
     pl.ctas = dev->sm_count;
     pl.least = 2;
-    pl.rows = tq * group;
+    // a CTA's work on an item of two query tiles begins and ends for as long as two tiles take; with one it is less, and in generation tiles are dearer
+    pl.extra = 2;
     pl.stride = p.T <= tq ? (p.T * group + 7) & ~7 : 2 * kTileQ;
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {

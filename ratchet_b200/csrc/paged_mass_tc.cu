@@ -321,18 +321,14 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
 // Adds the parts of tiles that several CTAs had, in their order (as merge_kernel).
 __global__ void __launch_bounds__(kTileK) mass_merge_kernel(const __grid_constant__ View p, const __grid_constant__ Plan pl) {
     rcu_kernel_entry();
-    const int W = pl.head[0], C = pl.head[1], b = blockIdx.x;
-    if (b + 1 >= C) return;
-    const long long total = (long long)W * p.G;
-    const int begin = first_tile(total, b, C), cut = first_tile(total, b + 1, C);
-    Walk wk(pl, b + 1, p.G, pl.head[2]);
-    const int start = wk.g * W + pl.prefix[wk.i], stop = wk.g * W + pl.prefix[wk.i + 1];
-    if (start == cut || start < begin) return;
+    const int b = blockIdx.x;
+    const Join jn(pl, b, p.G, pl.head[2]);
+    if (jn.count == 0) return;
     const float* parts = reinterpret_cast<const float*>(pl.ml);
-    const int r = threadIdx.x, j = wk.it.token * kTileK + r, L = clamp_int(p.lengths[wk.it.s], 0, p.MP << p.shift);
-    float sum = parts[(2 * b + (start != begin)) * kTileK + r];
-    for (int c = b + 1; c < C && first_tile(total, c, C) < stop; ++c) sum += parts[2 * c * kTileK + r];
-    if (j < L) p.mass[((size_t)wk.it.s * p.G + wk.g) * ((size_t)p.MP << p.shift) + j] += sum;
+    const int r = threadIdx.x, j = jn.it.token * kTileK + r, L = clamp_int(p.lengths[jn.it.s], 0, p.MP << p.shift);
+    float sum = 0.f;
+    for (int k = 0; k < jn.count; ++k) sum += parts[jn.slot(b, k) * kTileK + r];
+    if (j < L) p.mass[((size_t)jn.it.s * p.G + jn.g) * ((size_t)p.MP << p.shift) + j] += sum;
 }
 
 uint64_t mass_plan_of(const rcu_device* dev, const View& p, char* mem, Plan* out, int** base) {
