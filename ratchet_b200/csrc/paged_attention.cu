@@ -59,9 +59,12 @@ __global__ void __launch_bounds__(128) mass_kernel(const AttendArgs a) {
     p.mass[((size_t)s * p.G + g) * rows + j] += sum;
 }
 
-template <class T> rcu_status attend(rcu_device* dev, const AttendArgs& a, int dt, bool tc, void* scratch) {
+template <class T> rcu_status attend(rcu_device* dev, const AttendArgs& a, int dt, void* scratch) {
     const View& p = a.p;
-    if (tc) {
+    // both paths take a scale above zero, and queries and output that start on 16 bytes
+    const bool plain = !(a.c > 0.f) || !(a.c < INFINITY) || ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) != 0;
+    if (!plain && attend_rows_takes(dev, p, a.H, dt)) return attend_rows(dev, a, dt, scratch);
+    if (!plain && attend_tc_takes(dev, p, a.H, dt)) {
         // the two run one after the other: they share the scratch
         const rcu_status st = attend_tc(dev, a, dt, scratch);
         return st != RCU_OK || !p.mass ? st : mass_tc(dev, a, dt, scratch);
@@ -79,8 +82,9 @@ template <class T> rcu_status attend(rcu_device* dev, const AttendArgs& a, int d
 // lse of every query where mass is kept, and behind it what the tensor-core path takes (whether a call goes there is decided by more than the sizes)
 uint64_t lse_bytes(const View& p, uint64_t H) { return p.mass ? align256((uint64_t)p.T * H * 4) : 0; }
 uint64_t scratch_bytes(const rcu_device* dev, const View& p, uint64_t H, int dt) {
-    const bool tc = dt != RCU_F32 && p.D <= 128 && p.E <= 128 && H / p.G <= 128;
-    const uint64_t attend = tc ? attend_tc_scratch(dev, p, (int)H) : 0, mass = tc && p.mass ? mass_tc_scratch(dev, p, (int)H) : 0;
+    if (attend_rows_takes(dev, p, (int)H, dt)) return lse_bytes(p, H) + attend_rows_scratch(dev, p, (int)H, dt);
+    if (!attend_tc_takes(dev, p, (int)H, dt)) return lse_bytes(p, H);
+    const uint64_t attend = attend_tc_scratch(dev, p, (int)H), mass = p.mass ? mass_tc_scratch(dev, p, (int)H) : 0;
     return lse_bytes(p, H) + (attend > mass ? attend : mass);
 }
 
@@ -123,8 +127,7 @@ rcu_status rcu_paged_attention(rcu_device* dev, const rcu_tensor* q, const rcu_p
     if (st != RCU_OK) return st;
     a.lse = p.mass ? (float*)mem.ptr : nullptr;
     void* rest = (char*)mem.ptr + lse_bytes(p, H);
-    const bool tc = attend_tc_takes(dev, a, q->dt);
-    return q->dt == RCU_F32 ? attend<float>(dev, a, q->dt, tc, rest) : q->dt == RCU_F16 ? attend<__half>(dev, a, q->dt, tc, rest) : attend<__nv_bfloat16>(dev, a, q->dt, tc, rest);
+    return q->dt == RCU_F32 ? attend<float>(dev, a, q->dt, rest) : q->dt == RCU_F16 ? attend<__half>(dev, a, q->dt, rest) : attend<__nv_bfloat16>(dev, a, q->dt, rest);
 }
 
 }  // extern "C"

@@ -33,7 +33,7 @@ __device__ __forceinline__ void visible(int window, int first, int r, int& head,
 constexpr int kTileK = 128;
 
 struct Item {
-    int s, token, count, row;  // sequence; first token of the call, how many; row of the first one (s < 0: nothing to do)
+    int s, token, count, row;  // sequence; its first token of the item (in rows: first row of queries), how many; row of the first one
 };
 struct Plan {
     int items;                 // upper bound: T / tokens + S
@@ -153,7 +153,13 @@ struct Join {
 #endif
 
 // Any type, width and alignment (paged_attention.cu); f16 and bf16 up to 128 features on the tensor cores (paged_attention_tc.cu)
-bool attend_tc_takes(const rcu_device* dev, const AttendArgs& a, int dt);
+bool attend_tc_takes(const rcu_device* dev, const View& p, int H, int dt);
+// few rows per sequence, and f32 (paged_attention_rows.cu): sums the weights where mass is kept
+bool attend_rows_takes(const rcu_device* dev, const View& p, int H, int dt);
+uint64_t attend_rows_scratch(const rcu_device* dev, const View& p, int H, int dt);
+rcu_status attend_rows(rcu_device* dev, const AttendArgs& a, int dt, void* scratch);
+// launches plan_kernel: items of `plan.tokens` tokens, or of that many rows of queries where `group` of them make a token
+rcu_status plan_items(rcu_device* dev, const View& p, const Plan& plan, int window, int first, int group);
 uint64_t attend_tc_scratch(const rcu_device* dev, const View& p, int H);
 rcu_status attend_tc(rcu_device* dev, const AttendArgs& a, int dt, void* scratch);
 // the weights that every row receives, added to its mass; after the attention, whose lse it reads (paged_mass_tc.cu)

@@ -28,13 +28,8 @@ namespace {
 
 constexpr int kThreadsP = 384, kMostStages = 8;
 
-// whether one of the two 16-bit values is an infinity or NaN
-template <class T> __device__ __forceinline__ uint32_t not_finite(uint32_t x);
-template <> __device__ __forceinline__ uint32_t not_finite<__half>(uint32_t x) { return __vcmpgeu2(x & 0x7fff7fffu, 0x7c007c00u); }
-template <> __device__ __forceinline__ uint32_t not_finite<__nv_bfloat16>(uint32_t x) { return __vcmpgeu2(x & 0x7fff7fffu, 0x7f807f80u); }
-
 // One thread per item: its tokens and tiles; then the sums before each.  One CTA.
-__global__ void __launch_bounds__(1024) plan_kernel(const View p, const Plan pl, int window, int first) {
+__global__ void __launch_bounds__(1024) plan_kernel(const View p, const Plan pl, int window, int first, int group) {
     rcu_kernel_entry();
     __shared__ int warps[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -46,18 +41,19 @@ __global__ void __launch_bounds__(1024) plan_kernel(const View p, const Plan pl,
         Item it{-1, 0, 0, 0};
         int w = 0;
         if (i < pl.items) {
-            // sequence s has the items from starts[s] / tokens + s on
+            // sequence s has the items from starts[s] group / tokens + s on
+            auto begins = [&](int s, int start) { return (int)((long long)start * group / pl.tokens) + s; };
             int lo = 0, hi = p.S - 1;
             while (lo < hi) {
                 const int mid = (lo + hi + 1) / 2;
-                if (clamp_int(p.starts[mid], 0, p.T) / pl.tokens + mid <= i) lo = mid;
+                if (begins(mid, clamp_int(p.starts[mid], 0, p.T)) <= i) lo = mid;
                 else hi = mid - 1;
             }
             const Seq q = seq_of(p, lo);
-            const int at = (i - q.start / pl.tokens - lo) * pl.tokens;
-            if (at >= 0 && at < q.n) {
-                it = Item{lo, q.start + at, min(pl.tokens, q.n - at), q.old() + at};
-                w = span_of(window, first, it.row, min(it.row + it.count, q.L) - 1).count;
+            const long long at = (long long)(i - begins(lo, q.start)) * pl.tokens;
+            if (at >= 0 && at < (long long)q.n * group) {
+                it = Item{lo, (int)at, (int)min((long long)pl.tokens, (long long)q.n * group - at), q.old() + (int)at / group};
+                w = span_of(window, first, it.row, min(q.old() + ((int)at + it.count - 1) / group, q.L - 1)).count;
                 w += w > 0 ? pl.extra : 0;
             }
             pl.item[i] = it;
@@ -221,6 +217,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                     const Span sp = span_of(a.window, a.first, wk.it.row, wk.it.row + wk.it.count - 1);
                     const bool two = wk.it.count > x.tq;
                     seg.it = wk.it;
+                    seg.it.token += clamp_int(p.starts[wk.it.s], 0, p.T);
                     seg.g = wk.g;
                     seg.n0 = wk.n0;
                     seg.n1 = wk.n1;
@@ -627,7 +624,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Atte
     const int b = blockIdx.x;
     const Join jn(pl, b, p.G, pl.items);
     if (jn.count == 0) return;
-    const int rows = jn.it.count * group, quads = p.E / 4;
+    const int rows = jn.it.count * group, quads = p.E / 4, first_token = clamp_int(p.starts[jn.it.s], 0, p.T) + jn.it.token;
     for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += gridDim.y * 256) {
         const int u = i % rows, c = i / rows, token = u / group, h = jn.g * group + u % group;
         const int r = token / tq * kTileQ + u - token / tq * tq * group;
@@ -648,7 +645,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Atte
             o.w = fmaf(v.w, w, o.w);
         }
         const float inv = 1.f / l;
-        const size_t at = (size_t)(jn.it.token + token) * a.H + h;
+        const size_t at = (size_t)(first_token + token) * a.H + h;
         uint2 v;
         v.x = pack2<T>(o.x * inv, o.y * inv);
         v.y = pack2<T>(o.z * inv, o.w * inv);
@@ -695,8 +692,8 @@ template <class T> rcu_status launch(rcu_device* dev, const AttendArgs& a, int d
     CUtensorMap qm, km, vm;
     if (!map_queries(&qm, dt, p, a.q, x.group, x.tq) || !map_pages(&km, dt, p, p.keys, p.D) || !map_pages(&vm, dt, p, p.values, p.E))
         return rcu_fail(dev, RCU_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (%d tokens, %d heads, %d pages)", p.T, a.H, p.pages);
-    rcu_launch(dev, plan_kernel, 1, 1024, 0, p, x.pl, a.window, a.first);
-    RCU_LAUNCH_CHECK(dev);
+    const rcu_status planned = plan_items(dev, p, x.pl, a.window, a.first, 1);
+    if (planned != RCU_OK) return planned;
     void (*kern)(CUtensorMap, CUtensorMap, CUtensorMap, TcArgs) = paged_tc_kernel<T>;
     RCU_CUDA(dev, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     RCU_CUDA(dev, rcu_launch(dev, kern, x.pl.ctas, kThreadsP, smem, qm, km, vm, x));
@@ -712,12 +709,17 @@ template <class T> rcu_status launch(rcu_device* dev, const AttendArgs& a, int d
 
 }  // namespace
 
-bool attend_tc_takes(const rcu_device* dev, const AttendArgs& a, int dt) {
-    const View& p = a.p;
-    if (dt == RCU_F32 || p.D > 128 || p.E > 128 || a.H / p.G > kTileQ || !(a.c > 0.f) || !(a.c < INFINITY)) return false;
+rcu_status plan_items(rcu_device* dev, const View& p, const Plan& plan, int window, int first, int group) {
+    rcu_launch(dev, plan_kernel, 1, 1024, 0, p, plan, window, first, group);
+    RCU_LAUNCH_CHECK(dev);
+    return RCU_OK;
+}
+
+bool attend_tc_takes(const rcu_device* dev, const View& p, int H, int dt) {
+    const int group = H / p.G;
+    if (dt == RCU_F32 || p.D > 128 || p.E > 128 || group > kTileQ || dev->smem_optin < 227 * 1024) return false;
     // 32-bit tile numbers: all kv heads' tiles over the longest rows that the table allows
-    if ((uint64_t)(p.T / (kTileQ / (a.H / p.G)) + p.S) * (((uint64_t)p.MP << p.shift) / kTileK + 1) * p.G >= (1ull << 31)) return false;
-    return ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 && dev->smem_optin >= 227 * 1024;
+    return (uint64_t)(p.T / (kTileQ / group) + p.S) * (((uint64_t)p.MP << p.shift) / kTileK + 3) * p.G < (1ull << 31);
 }
 
 uint64_t attend_tc_scratch(const rcu_device* dev, const View& p, int H) { return plan_of(dev, p, H, nullptr, nullptr); }

@@ -25,6 +25,11 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
     const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// whether one of the two 16-bit values is an infinity or NaN
+template <class T> __device__ __forceinline__ uint32_t not_finite(uint32_t x);
+template <> __device__ __forceinline__ uint32_t not_finite<__half>(uint32_t x) { return __vcmpgeu2(x & 0x7fff7fffu, 0x7c007c00u); }
+template <> __device__ __forceinline__ uint32_t not_finite<__nv_bfloat16>(uint32_t x) { return __vcmpgeu2(x & 0x7fff7fffu, 0x7f807f80u); }
+
 // two f32 operations of one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -144,27 +149,29 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_u32(bar))
                  : "memory");
 }
-// [pages or tokens, heads, rows, features] of 16 bits, boxes of 64 features; 128-byte swizzle, what lies beyond the extents reads as zero
+// [pages or tokens, heads, rows, features], boxes of 128 bytes of features; 128-byte swizzle, what lies beyond the extents reads as zero
 inline bool map_4d(CUtensorMap* map, int dt, const void* base, const uint64_t (&dims)[4], uint32_t box1, uint32_t box3) {
     gemvq8::EncodeTiledFn fn = gemvq8::encode_tiled_fn();
     if (!fn) return false;
+    const uint64_t e = dt_esize(dt);
     cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
-    cuuint64_t strides[3] = {dims[0] * 2, dims[0] * dims[1] * 2, dims[0] * dims[1] * dims[2] * 2};
-    cuuint32_t box[4] = {64, box1, 1, box3};
+    cuuint64_t strides[3] = {dims[0] * e, dims[0] * dims[1] * e, dims[0] * dims[1] * dims[2] * e};
+    cuuint32_t box[4] = {(cuuint32_t)(128 / e), box1, 1, box3};
     cuuint32_t estr[4] = {1, 1, 1, 1};
-    return fn(map, dt == RCU_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), d, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const CUtensorMapDataType type = dt == RCU_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : dt == RCU_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    return fn(map, type, 4, const_cast<void*>(base), d, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
 
 // queries by tiles of `tq` tokens with the heads of a group, and rows of pages by 128 or by whole pages
 inline bool map_queries(CUtensorMap* map, int dt, const View& p, const void* q, int group, int tq) {
     const uint64_t d[4] = {(uint64_t)p.D, (uint64_t)group, (uint64_t)p.G, (uint64_t)p.T};
     return map_4d(map, dt, q, d, group, tq);
 }
-inline bool map_pages(CUtensorMap* map, int dt, const View& p, const void* pages, int width) {
+inline bool map_slices(CUtensorMap* map, int dt, const View& p, const void* pages, int width, int rows) {
     const uint64_t d[4] = {(uint64_t)width, (uint64_t)p.R, (uint64_t)p.G, (uint64_t)p.pages};
-    return map_4d(map, dt, pages, d, p.R < kTileK ? p.R : kTileK, 1);
+    return map_4d(map, dt, pages, d, rows, 1);
 }
+inline bool map_pages(CUtensorMap* map, int dt, const View& p, const void* pages, int width) { return map_slices(map, dt, p, pages, width, p.R < kTileK ? p.R : kTileK); }
 
 }  // namespace paged
