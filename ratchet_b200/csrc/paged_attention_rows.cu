@@ -18,10 +18,10 @@ namespace {
 constexpr int kSlice = 16, kRing = 3;
 
 template <class T> struct Form {
-    static constexpr int kWarps = 8, kRows = 16, kCols = 64;          // columns of 128 bytes
+    static constexpr int kRows = 16, kCols = 64;          // columns of 128 bytes
 };
 template <> struct Form<float> {
-    static constexpr int kWarps = 4, kRows = 8, kCols = 32;
+    static constexpr int kRows = 8, kCols = 32;
 };
 
 struct RowsArgs {
@@ -245,10 +245,10 @@ template <> struct Part<float> {
     }
 };
 
-template <class T>
-__global__ void __launch_bounds__(Form<T>::kWarps * 32, 1)
+template <class T, int W>
+__global__ void __launch_bounds__(W * 32, 1)
 rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ RowsArgs x) {
-    constexpr int W = Form<T>::kWarps, BQ = Form<T>::kRows, C = Form<T>::kCols;
+    constexpr int BQ = Form<T>::kRows, C = Form<T>::kCols;
     constexpr bool f32 = sizeof(T) == 4;
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(8) uint64_t full[W][kRing];
@@ -280,10 +280,12 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         const Span sp = span_of(a.window, a.first, r0, r1);
         const int end = min(L, r1 + 1), slices = (wk.n1 - wk.n0) * (kTileK / kSlice / W);
         auto slice_at = [&](int i) { return sp.tile(wk.n0 + i / (kTileK / kSlice / W)) * kTileK + (i % (kTileK / kSlice / W) * W + warp) * kSlice; };
+        PageIds ids;
+        const int have = min(p.MP, (L + p.R - 1) >> p.shift);
         auto ask = [&](int i) {
             const int j = slice_at(i);
             if (j >= end || !ok) return;
-            const int page = page_of(p, s, j), st = asked % kRing;
+            const int at = j >> p.shift, page = ids.of(p, s, at, at, at, have), st = asked % kRing;
             if (lane == 0) {
                 unsigned char* to = ring + st * slot_bytes;
                 mbar_expect_tx(&full[warp][st], slot_bytes);
@@ -405,38 +407,51 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     }
 }
 
-// As merge_kernel of paged_attention_tc.cu, for items of rows
+// As merge_kernel of paged_attention_tc.cu, for items of rows: the parts' factors first, in shared memory, then their sums
 template <class T>
-__global__ void __launch_bounds__(128) rows_merge_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan pl, int group) {
+__global__ void __launch_bounds__(256) rows_merge_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan pl, int group) {
+    constexpr int BQ = Form<T>::kRows;
     rcu_kernel_entry();
+    extern __shared__ float factor[];          // [parts][BQ]
+    __shared__ float total[BQ];
     const View& p = a.p;
     const int b = blockIdx.x;
     const Join jn(pl, b, p.G, pl.items);
     if (jn.count == 0) return;
-    const int start = clamp_int(p.starts[jn.it.s], 0, p.T), quads = p.E / 4;
-    for (int i = threadIdx.x; i < jn.it.count * quads; i += 128) {
-        const int u = i % jn.it.count, c = i / jn.it.count, f = jn.it.token + u, h = jn.g * group + f % group;
-        const size_t q = (size_t)(start + f / group) * a.H + h;
-        float m = -INFINITY;
-#pragma unroll 4
-        for (int k = 0; k < jn.count; ++k) m = fmaxf(m, pl.ml[(size_t)jn.slot(b, k) * pl.stride + u].x);
-        const float sk = a.sink ? a.sink[h] * kLog2e : -INFINITY, top = fmaxf(m, sk);
-        float l = a.sink ? ex2(sk - top) : 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int k = 0; k < jn.count; ++k) {
+    const int start = clamp_int(p.starts[jn.it.s], 0, p.T), quads = p.E / 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int u = warp; u < jn.it.count; u += 8) {
+        const int f = jn.it.token + u, h = jn.g * group + f % group;
+        float m = a.sink ? a.sink[h] * kLog2e : -INFINITY;
+        const float sk = m;
+        for (int k = lane; k < jn.count; k += 32) m = fmaxf(m, pl.ml[(size_t)jn.slot(b, k) * pl.stride + u].x);
+        m = warp_max(m);
+        float l = 0.f;
+        for (int k = lane; k < jn.count; k += 32) {
             const float2 ml = pl.ml[(size_t)jn.slot(b, k) * pl.stride + u];
-            const float4 v = pl.o[((size_t)jn.slot(b, k) * quads + c) * pl.stride + u];
-            const bool none = ml.x == -INFINITY && ml.y == 0.f;          // a part that sees nothing has no sum
-            const float w = none ? 0.f : ex2(ml.x - top);
+            const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2(ml.x - m);          // a part that sees nothing has no sum
+            factor[k * BQ + u] = w;
             l = fmaf(ml.y, w, l);
+        }
+        l = warp_sum(l) + (a.sink ? ex2(sk - m) : 0.f);
+        if (lane == 0) {
+            total[u] = 1.f / l;
+            if (a.lse) a.lse[(size_t)(start + f / group) * a.H + h] = m + log2f(l);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < jn.it.count * quads; i += 256) {
+        const int u = i % jn.it.count, c = i / jn.it.count, f = jn.it.token + u, h = jn.g * group + f % group;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int k = 0; k < jn.count; ++k) {
+            const float4 v = pl.o[((size_t)jn.slot(b, k) * quads + c) * pl.stride + u];
+            const float w = factor[k * BQ + u];
             o = make_float4(fmaf(v.x, w, o.x), fmaf(v.y, w, o.y), fmaf(v.z, w, o.z), fmaf(v.w, w, o.w));
         }
-        const float inv = 1.f / l;
-        T* out = (T*)a.out + q * p.E + 4 * c;
+        const float inv = total[u];
+        T* out = (T*)a.out + ((size_t)(start + f / group) * a.H + h) * p.E + 4 * c;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
-        if (a.lse && c == 0) a.lse[q] = top + log2f(l);
     }
 }
 
@@ -489,7 +504,7 @@ uint64_t rows_plan_of(const rcu_device* dev, const View& p, int H, int dt, char*
 
 template <class T> rcu_status launch_rows(rcu_device* dev, const AttendArgs& a, int dt, void* scratch) {
     const View& p = a.p;
-    constexpr int W = Form<T>::kWarps, C = Form<T>::kCols;
+    constexpr int C = Form<T>::kCols;
     RowsArgs x{a, {}, a.H / p.G, (p.D + C - 1) / C, (p.E + C - 1) / C, nullptr};
     rows_plan_of(dev, p, a.H, dt, (char*)scratch, &x.pl, &x.scores);
     if (!p.mass) x.scores = nullptr;
@@ -498,14 +513,16 @@ template <class T> rcu_status launch_rows(rcu_device* dev, const AttendArgs& a, 
         return rcu_fail(dev, RCU_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (%d tokens, %d heads, %d pages)", p.T, a.H, p.pages);
     rcu_status st = plan_items(dev, p, x.pl, a.window, a.first, x.group);
     if (st != RCU_OK) return st;
-    const size_t ring = (size_t)W * kRing * (x.nb + x.eb) * kSlice * 128, sums = (size_t)W * Form<T>::kRows * p.E * 4;
-    const size_t smem = 1024 + (ring > sums ? ring : sums);
-    void (*kern)(CUtensorMap, CUtensorMap, RowsArgs) = rows_kernel<T>;
+    // eight warps where their rings fit, which is always in 16 bits
+    const size_t warp_ring = (size_t)kRing * (x.nb + x.eb) * kSlice * 128, warp_sums = (size_t)Form<T>::kRows * p.E * 4;
+    const int warps = 8 * warp_ring <= 192 * 1024 ? 8 : 4;
+    const size_t smem = 1024 + warps * (warp_ring > warp_sums ? warp_ring : warp_sums);
+    void (*kern)(CUtensorMap, CUtensorMap, RowsArgs) = warps == 8 ? rows_kernel<T, 8> : rows_kernel<T, sizeof(T) == 4 ? 4 : 8>;
     RCU_CUDA(dev, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    RCU_CUDA(dev, rcu_launch(dev, kern, x.pl.ctas, W * 32, smem, km, vm, x));
+    RCU_CUDA(dev, rcu_launch(dev, kern, x.pl.ctas, warps * 32, smem, km, vm, x));
     RCU_LAUNCH_CHECK(dev);
     if (x.pl.ctas > 1) {
-        rcu_launch(dev, rows_merge_kernel<T>, x.pl.ctas - 1, 128, 0, a, x.pl, x.group);
+        rcu_launch(dev, rows_merge_kernel<T>, x.pl.ctas - 1, 256, (size_t)x.pl.ctas * Form<T>::kRows * 4, a, x.pl, x.group);
         RCU_LAUNCH_CHECK(dev);
     }
     if (p.mass) {

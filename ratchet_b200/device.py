@@ -19,7 +19,7 @@ from .capi import RatchetCudaError
 class Buffer:
     """A resolved tensor on the device: dtype, logical shape and one pooled allocation."""
 
-    __slots__ = ("dev", "dt", "shape", "ptr", "nbytes", "_owned", "_base")
+    __slots__ = ("dev", "dt", "shape", "ptr", "nbytes", "_owned", "_base", "_byref")
 
     def __init__(self, dev: "Device", dt: int, shape, ptr: int, nbytes: int, owned: bool, base=None):
         self.dev = dev
@@ -29,6 +29,7 @@ class Buffer:
         self.nbytes = nbytes
         self._owned = owned
         self._base = base  # keeps the owning buffer alive for views
+        self._byref = None  # reference to a descriptor, made by the first call that takes this buffer
 
     @property
     def numel(self) -> int:
@@ -64,6 +65,7 @@ class Buffer:
             self.dev._free(self.ptr)
             self.ptr = 0
             self._owned = False
+            self._byref = None
 
     def __del__(self):
         try:
@@ -192,7 +194,12 @@ class Device:
 
     # ------------------------------------------------------------------ ops (eager, one C-ABI call each)
     def _ref(self, b: Optional[Buffer]):
-        return None if b is None else C.byref(b.desc())
+        """A descriptor of the buffer for the C ABI, which only reads it.  Kept by the buffer: making one takes longer than a short kernel runs."""
+        if b is None:
+            return None
+        if b._byref is None:
+            b._byref = C.byref(b.desc())
+        return b._byref
 
     def dequantize(self, src: Buffer, out: Optional[Buffer] = None) -> Buffer:
         out = out or self.empty(capi.activation_dtype(src.dt), src.shape)
