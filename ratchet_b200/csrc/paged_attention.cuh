@@ -50,6 +50,8 @@ struct Plan {
 };
 
 #ifdef __CUDACC__
+struct Span;
+__device__ __forceinline__ Span span_of(int window, int first, int r0, int r1);
 // Tiles that tokens at rows r0 .. r1 see: the first `head` ones, then lo, lo + 1, ..
 struct Span {
     int head, lo, count;
@@ -65,17 +67,80 @@ __device__ __forceinline__ Span span_of(int window, int first, int r0, int r1) {
     return sp;
 }
 
+// A call's items and where they begin, into pl.head, pl.prefix and pl.item, by a CTA of THREADS threads.  One thread per item; `starts` (nullable) has room
+// for the sequences' starts in shared memory, where looking for an item's sequence takes no time.
+template <int THREADS>
+__device__ __forceinline__ void plan_items_block(const View& p, const Plan& pl, int window, int first, int group, int* starts) {
+    __shared__ int warps[THREADS / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (starts) {
+        for (int s = tid; s < p.S; s += THREADS) starts[s] = clamp_int(p.starts[s], 0, p.T);
+        __syncthreads();
+    }
+    int before = 0;
+#pragma unroll 1
+    for (int base = 0; base < pl.items; base += THREADS) {
+        const int i = base + tid;
+        Item it{-1, 0, 0, 0};
+        int w = 0;
+        if (i < pl.items) {
+            // sequence s has the items from starts[s] group / tokens + s on
+            auto begins = [&](int s) { return (int)((long long)(starts ? starts[s] : clamp_int(p.starts[s], 0, p.T)) * group / pl.tokens) + s; };
+            int lo = 0, hi = p.S - 1;
+#pragma unroll 1
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (begins(mid) <= i) lo = mid;
+                else hi = mid - 1;
+            }
+            const Seq q = seq_of(p, lo);
+            const long long at = (long long)(i - begins(lo)) * pl.tokens;
+            if (at >= 0 && at < (long long)q.n * group) {
+                it = Item{lo, (int)at, (int)min((long long)pl.tokens, (long long)q.n * group - at), q.old() + (int)at / group};
+                w = span_of(window, first, it.row, min(q.old() + ((int)at + it.count - 1) / group, q.L - 1)).count;
+                w += w > 0 ? pl.extra : 0;
+            }
+            pl.item[i] = it;
+        }
+        int upto = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 31) warps[warp] = upto;
+        __syncthreads();
+        int add = before, all = 0;
+#pragma unroll 4
+        for (int j = 0; j < THREADS / 32; ++j) {
+            if (j < warp) add += warps[j];
+            all += warps[j];
+        }
+        if (i < pl.items) pl.prefix[i] = add + upto - w;
+        before += all;
+        __syncthreads();
+    }
+    if (tid == 0) {
+        pl.prefix[pl.items] = before;
+        pl.head[0] = before;
+        const long long total = (long long)before * p.G;
+        pl.head[1] = (int)max(1ll, min((long long)pl.ctas, (total + pl.least - 1) / pl.least));
+    }
+    __syncthreads();
+}
+
 // The tiles that CTA b of C takes of `total`
 __device__ __forceinline__ int first_tile(long long total, int b, int C) { return (int)(total * b / C); }
 
-// The item at place y of a kv head's row
+// The item at place y of a kv head's row, by whole warps: 32 places are looked at per step
 __device__ __forceinline__ int item_at(const Plan& pl, int items, int y) {
     int lo = 0, hi = items - 1;                  // the last item that begins there or before
 #pragma unroll 1
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (pl.prefix[mid] <= y) lo = mid;
-        else hi = mid - 1;
+    while (hi > lo) {
+        const int step = (hi - lo + 31) / 32, at = lo + ((int)(threadIdx.x & 31) + 1) * step;
+        const int k = __popc(__ballot_sync(0xffffffffu, at <= hi && pl.prefix[min(at, hi)] <= y));
+        hi = min(hi, lo + (k + 1) * step - 1);
+        lo += k * step;
     }
     return lo;
 }
@@ -145,8 +210,7 @@ struct Join {
         const int i = item_at(pl, items, cut - g * W), p0 = g * W + pl.prefix[i] + pl.extra, p1 = g * W + pl.prefix[i + 1];
         if (cut <= p0 || before > p0) return;
         it = pl.item[i];
-        count = 1;
-        while (b + count < C && first_tile(total, b + count, C) < p1) ++count;
+        count = (int)min((long long)C, ((long long)p1 * C + total - 1) / total) - b;          // CTAs from b on that begin before p1
     }
     __device__ __forceinline__ int slot(int b, int k) const { return k == 0 ? 2 * b + 1 : 2 * (b + k); }
 };

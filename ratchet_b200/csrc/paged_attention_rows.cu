@@ -15,7 +15,7 @@
 namespace paged {
 namespace {
 
-constexpr int kSlice = 16, kRing = 3;
+constexpr int kSlice = 16, kRing = 3, kPlanned = 256;
 
 template <class T> struct Form {
     static constexpr int kRows = 16, kCols = 64;          // columns of 128 bytes
@@ -28,6 +28,7 @@ struct RowsArgs {
     AttendArgs a;
     Plan pl;
     int group, nb, eb;         // query heads of a kv head; 128-byte blocks of a key and of a value
+    int plans;                 // the kernel works the items out itself (kPlanned at most), and leaves them for the next one
     float* scores;             // [T * H, MP * R]: scores in units of log 2, where mass is kept
 };
 
@@ -269,10 +270,29 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     }
     __syncthreads();
     rcu_kernel_entry_wait_only();          // nothing before this touches global memory
+    // Few items are worked out by every CTA for itself: a kernel of one CTA in front of this one took 3 us
+    __shared__ int starts[kPlanned], prefix[kPlanned + 1], head[2];
+    __shared__ Item items[kPlanned];
+    Plan pl = x.pl;
+    if (x.plans) {
+        pl.head = head;
+        pl.prefix = prefix;
+        pl.item = items;
+        plan_items_block<W * 32>(p, pl, a.window, a.first, x.group, starts);
+        if (blockIdx.x == 0) {
+            for (int s = threadIdx.x; s < p.S; s += W * 32)
+                if (seq_bad(p, s)) report_bad(p.status);
+            for (int i = threadIdx.x; i <= pl.items; i += W * 32) {
+                x.pl.prefix[i] = prefix[i];
+                if (i < pl.items) x.pl.item[i] = items[i];
+                if (i < 2) x.pl.head[i] = head[i];
+            }
+        }
+    }
     bool ok = true;
     int asked = 0, had = 0, turn = 0;      // slices so far; parity of the part
 #pragma unroll 1
-    for (Walk wk(x.pl, blockIdx.x, p.G, x.pl.items); wk.more(); wk.next(), turn ^= 1) {
+    for (Walk wk(pl, blockIdx.x, p.G, pl.items); wk.more(); wk.next(), turn ^= 1) {
         // rows f0 .. f0 + count - 1 of the sequence's queries: token f / group, head f % group
         const Seq sq = seq_of(p, wk.it.s);
         const int f0 = wk.it.token, count = wk.it.count, g = wk.g, s = wk.it.s;
@@ -505,14 +525,17 @@ uint64_t rows_plan_of(const rcu_device* dev, const View& p, int H, int dt, char*
 template <class T> rcu_status launch_rows(rcu_device* dev, const AttendArgs& a, int dt, void* scratch) {
     const View& p = a.p;
     constexpr int C = Form<T>::kCols;
-    RowsArgs x{a, {}, a.H / p.G, (p.D + C - 1) / C, (p.E + C - 1) / C, nullptr};
+    RowsArgs x{a, {}, a.H / p.G, (p.D + C - 1) / C, (p.E + C - 1) / C, 0, nullptr};
     rows_plan_of(dev, p, a.H, dt, (char*)scratch, &x.pl, &x.scores);
     if (!p.mass) x.scores = nullptr;
     CUtensorMap km, vm;
     if (!map_slices(&km, dt, p, p.keys, p.D, kSlice) || !map_slices(&vm, dt, p, p.values, p.E, kSlice))
         return rcu_fail(dev, RCU_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (%d tokens, %d heads, %d pages)", p.T, a.H, p.pages);
-    rcu_status st = plan_items(dev, p, x.pl, a.window, a.first, x.group);
-    if (st != RCU_OK) return st;
+    x.plans = x.pl.items <= kPlanned && p.S <= kPlanned;
+    if (!x.plans) {
+        const rcu_status st = plan_items(dev, p, x.pl, a.window, a.first, x.group);
+        if (st != RCU_OK) return st;
+    }
     // eight warps where their rings fit, which is always in 16 bits
     const size_t warp_ring = (size_t)kRing * (x.nb + x.eb) * kSlice * 128, warp_sums = (size_t)Form<T>::kRows * p.E * 4;
     const int warps = 8 * warp_ring <= 192 * 1024 ? 8 : 4;

@@ -28,59 +28,12 @@ namespace {
 
 constexpr int kThreadsP = 384, kMostStages = 8;
 
-// One thread per item: its tokens and tiles; then the sums before each.  One CTA.
-__global__ void __launch_bounds__(1024) plan_kernel(const View p, const Plan pl, int window, int first, int group) {
+__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ View p, const __grid_constant__ Plan pl, int window, int first, int group) {
     rcu_kernel_entry();
-    __shared__ int warps[32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int s = tid; s < p.S; s += 1024)
+    __shared__ int starts[2048];
+    for (int s = threadIdx.x; s < p.S; s += 1024)
         if (seq_bad(p, s)) report_bad(p.status);
-    int before = 0;
-    for (int base = 0; base < pl.items; base += 1024) {
-        const int i = base + tid;
-        Item it{-1, 0, 0, 0};
-        int w = 0;
-        if (i < pl.items) {
-            // sequence s has the items from starts[s] group / tokens + s on
-            auto begins = [&](int s, int start) { return (int)((long long)start * group / pl.tokens) + s; };
-            int lo = 0, hi = p.S - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (begins(mid, clamp_int(p.starts[mid], 0, p.T)) <= i) lo = mid;
-                else hi = mid - 1;
-            }
-            const Seq q = seq_of(p, lo);
-            const long long at = (long long)(i - begins(lo, q.start)) * pl.tokens;
-            if (at >= 0 && at < (long long)q.n * group) {
-                it = Item{lo, (int)at, (int)min((long long)pl.tokens, (long long)q.n * group - at), q.old() + (int)at / group};
-                w = span_of(window, first, it.row, min(q.old() + ((int)at + it.count - 1) / group, q.L - 1)).count;
-                w += w > 0 ? pl.extra : 0;
-            }
-            pl.item[i] = it;
-        }
-        int upto = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        if (lane == 31) warps[warp] = upto;
-        __syncthreads();
-        int add = before, all = 0;
-        for (int j = 0; j < 32; ++j) {
-            if (j < warp) add += warps[j];
-            all += warps[j];
-        }
-        if (i < pl.items) pl.prefix[i] = add + upto - w;
-        before += all;
-        __syncthreads();
-    }
-    if (tid == 0) {
-        pl.prefix[pl.items] = before;
-        pl.head[0] = before;
-        const long long total = (long long)before * p.G;
-        pl.head[1] = (int)max(1ll, min((long long)pl.ctas, (total + pl.least - 1) / pl.least));
-    }
+    plan_items_block<1024>(p, pl, window, first, group, p.S <= 2048 ? starts : nullptr);
 }
 
 struct TcArgs {
