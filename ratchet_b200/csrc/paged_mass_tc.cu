@@ -16,7 +16,7 @@
 namespace paged {
 namespace {
 
-constexpr int kThreadsM = 320, kStagesQ = 4;
+constexpr int kThreadsM = 320, kStagesQ = 4, kStagesL = 8;       // query tiles in shared memory; their lse, which are read for longer
 
 // Query tiles j of sequence q (tq tokens each) that see any of the rows j0 .. j0 + 127: [lo, hi)
 __device__ __forceinline__ void seen_by(const Seq& q, int window, int first, int tq, int j0, int& lo, int& hi) {
@@ -107,10 +107,9 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
     const int tile_bytes = x.nb * kBlock;
     unsigned char* ks = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
     unsigned char* ring = ks + 2 * tile_bytes;
-    __shared__ __align__(16) float lse[kStagesQ][kTileQ];
-    __shared__ __align__(16) int rows[kStagesQ][kTileQ];              // of the queries; -1: none
+    __shared__ __align__(16) float lse[kStagesL][kTileQ];             // -lse of a tile's queries, -infinity where there is none
     __shared__ float sums[2][kTileK];
-    __shared__ __align__(8) uint64_t k_full[2], k_empty[2], q_full[kStagesQ], q_empty[kStagesQ], s_full[4], s_empty[4], handed[2], taken[2], drained;
+    __shared__ __align__(8) uint64_t k_full[2], k_empty[2], q_full[kStagesQ], q_empty[kStagesQ], l_full[kStagesL], l_empty[kStagesL], s_full[4], s_empty[4], handed[2], taken[2], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
 
@@ -124,8 +123,12 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
             mbar_init(&taken[i], 4);
         }
         for (int i = 0; i < kStagesQ; ++i) {
-            mbar_init(&q_full[i], 33);
-            mbar_init(&q_empty[i], 5);           // the product's, and the four warps that read the lse
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], 1);
+        }
+        for (int i = 0; i < kStagesL; ++i) {
+            mbar_init(&l_full[i], 32);
+            mbar_init(&l_empty[i], 4);           // of the group that has the tile
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
@@ -151,93 +154,120 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
     rcu_kernel_entry_wait_only();        // nothing before this touches global memory
     const uint32_t tmem = tmem_slot;
     const int items = x.pl.head[2];
+    auto wait = [&](uint64_t* bar, int phase) { return wait_warp(bar, phase, &abort_flag, p.status); };
 
     if (warp == 0) {
         const int rows_box = min(p.R, kTileK), boxes = kTileK / rows_box, box = lane % boxes, col = lane / boxes;
+        // this lane's four queries of a tile: token and head
+        int token[4], head[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int u = lane + 32 * i;
+            token[i] = u < filled ? u / x.group : 1 << 30;
+            head[i] = u % x.group;
+        }
         int item = 0, fills = 0;
+        RingAt at{kStagesQ, 0, 0}, lat{kStagesL, 0, 0};
         bool ok = true;
+#pragma unroll 1
         for (Walk wk(x.pl, blockIdx.x, p.G, items); wk.more() && ok; wk.next(), ++item) {
             const Seq q = seq_of(p, wk.it.s);
             const int j0 = wk.it.token * kTileK, b = item & 1;
             const int page = j0 + box * rows_box < q.L ? page_of(p, wk.it.s, j0 + box * rows_box) : -1;
             const int pages = __popc(__ballot_sync(0xffffffffu, lane < boxes && page >= 0));
-            if (item >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[b], (item / 2 - 1) & 1, &abort_flag, p.status));
+            ok = wait(&k_empty[b], (item / 2) ^ 1);
             if (!ok) break;
             if (lane == 0) mbar_expect_tx(&k_full[b], pages * x.nb * rows_box * 128);
             __syncwarp();
             if (lane < boxes * x.nb && page >= 0) tma_load_4d(ks + b * tile_bytes + col * kBlock + box * rows_box * 128, &kmap, col * 64, j0 & (p.R - 1), wk.g, page, &k_full[b]);
-            for (int n = wk.n0; n < wk.n1 && ok; ++n, ++fills) {
-                const int s = fills % kStagesQ, t0 = (wk.it.count + n) * x.tq;
-                float v[4];
-                int r[4];
+            // the lse of a tile's queries is asked for while the tile before goes its way
+            auto ask = [&](int n, float (&v)[4]) {
+                const int t0 = (wk.it.count + n) * x.tq;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int u = lane + 32 * i, t = t0 + u / x.group;
-                    const bool in = u < filled && t < q.n;
-                    v[i] = in ? a.lse[(size_t)(q.start + t) * a.H + wk.g * x.group + u % x.group] : INFINITY;
-                    r[i] = in ? q.old() + t : -1;
+                    const bool in = token[i] < q.n - t0;
+                    v[i] = in ? a.lse[(size_t)(q.start + t0 + token[i]) * a.H + wk.g * x.group + head[i]] : INFINITY;
                 }
-                if (fills >= kStagesQ) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[s], (fills / kStagesQ - 1) & 1, &abort_flag, p.status));
+            };
+            float v[4];
+            ask(wk.n0, v);
+#pragma unroll 1
+            for (int n = wk.n0; n < wk.n1; ++n, ++fills) {
+                const int t0 = (wk.it.count + n) * x.tq;
+                float next[4] = {0.f, 0.f, 0.f, 0.f};
+                if (n + 1 < wk.n1) ask(n + 1, next);
+                ok = wait(&q_empty[at.s], at.phase ^ 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    mbar_expect_tx(&q_full[at.s], x.nb * filled * 128);
+#pragma unroll 1
+                    for (int c = 0; c < x.nb; ++c) tma_load_4d(ring + (size_t)at.s * tile_bytes + c * kBlock, &qmap, c * 64, 0, wk.g, q.start + t0, &q_full[at.s]);
+                }
+                __syncwarp();
+                ok = wait(&l_empty[lat.s], lat.phase ^ 1);
                 if (!ok) break;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    lse[s][lane + 32 * i] = v[i];
-                    rows[s][lane + 32 * i] = r[i];
+                    lse[lat.s][lane + 32 * i] = -v[i];
+                    v[i] = next[i];
                 }
-                mbar_arrive(&q_full[s]);
-                if (lane == 0) {
-                    mbar_expect_tx(&q_full[s], x.nb * filled * 128);
-                    for (int c = 0; c < x.nb; ++c) tma_load_4d(ring + (size_t)s * tile_bytes + c * kBlock, &qmap, c * 64, 0, wk.g, q.start + t0, &q_full[s]);
-                }
+                mbar_arrive(&l_full[lat.s]);
+                lat.go(1);
                 __syncwarp();
+                at.go(1);
             }
         }
         if (!ok) {          // given up: let the copies in flight land before the memory is somebody else's
-            for (int i = max(0, fills - kStagesQ); i < fills; ++i)
-                for (int k = 0; k < (1 << 16) && !gemvq8::mbar_test_wait(&q_full[i % kStagesQ], (i / kStagesQ) & 1); ++k) {}
-            for (int i = max(0, item - 1); i <= item; ++i)
-                for (int k = 0; k < (1 << 16) && !gemvq8::mbar_test_wait(&k_full[i & 1], (i / 2) & 1); ++k) {}
+#pragma unroll 1
+            for (int i = max(0, fills - kStagesQ); i <= fills; ++i) land(&q_full[i % kStagesQ], i / kStagesQ);
+#pragma unroll 1
+            for (int i = max(0, item - 1); i <= item; ++i) land(&k_full[i & 1], i / 2);
         }
     } else if (warp == 1) {
+        // one lane: what it does between two products, tensor memory waits for.  Every lane walks, one goes on.
+        const bool leader = elect_one();
         constexpr bool bf16 = !std::is_same<T, __half>::value;
         const uint32_t idesc = umma_idesc_f16(kTileK, kTileQ, bf16);
-        const int ksteps = (p.D + 15) / 16;
+        const int ksteps = (p.D + 15) / 16, tile16 = tile_bytes >> 4;
         const uint64_t kd = umma_desc_sw128(ks), qd = umma_desc_sw128(ring);
-        const bool leader = elect_one();
-        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, &abort_flag, p.status)); };
+        auto wait1 = [&](uint64_t* bar, int phase) { return gemvq8::mbar_try_wait(bar, phase & 1) || wait_on(bar, phase & 1, &abort_flag, p.status); };
         bool ok = true;
-        int item = 0, at = 0;                    // at: query tiles so far
+        int item = 0, done = 0;                    // done: query tiles so far
+        RingAt at{kStagesQ, 0, 0};
+#pragma unroll 1
         for (Walk wk(x.pl, blockIdx.x, p.G, items); wk.more() && ok; wk.next(), ++item) {
             const int b = item & 1;
-            ok = wait(&k_full[b], item / 2);
-            for (int n = wk.n0; n < wk.n1 && ok; ++n, ++at) {
-                const int s = at % kStagesQ, t = at & 3;
-                ok = wait(&q_full[s], at / kStagesQ);
-                if (ok && at >= 4) ok = wait(&s_empty[t], at / 4 - 1);
-                if (!ok) break;
-                tc_fence_after();
-                if (leader) {
-                    const uint64_t ad = kd + (uint64_t)(b * (tile_bytes >> 4)), bd = qd + (uint64_t)(s * (tile_bytes >> 4));
-                    for (int k = 0; k < ksteps; ++k) {
-                        const uint64_t off = (k >> 2) * (kBlock >> 4) + 2 * (k & 3);
-                        umma_f16(tmem + 128 * t, ad + off, bd + off, idesc, k > 0 ? 1u : 0u);
-                    }
+            if (leader) {
+                ok = wait1(&k_full[b], item / 2);
+#pragma unroll 1
+                for (int n = wk.n0; n < wk.n1 && ok; ++n) {
+                    const int t = done & 3;
+                    ok = wait1(&q_full[at.s], at.phase) && wait1(&s_empty[t], (done / 4) ^ 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t ad = kd + (uint64_t)(b * tile16), bd = qd + (uint64_t)(at.s * tile16);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k < ksteps) umma_f16(tmem + 128 * t, ad + (k >> 2) * (kBlock >> 4) + 2 * (k & 3), bd + (k >> 2) * (kBlock >> 4) + 2 * (k & 3), idesc, k > 0 ? 1u : 0u);
                     umma_commit(&s_full[t]);
-                    umma_commit(&q_empty[s]);
+                    umma_commit(&q_empty[at.s]);
                     if (n == wk.n1 - 1) umma_commit(&k_empty[b]);
+                    ++done;
+                    at.go(1);
                 }
-                __syncwarp();
             }
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok && leader) {            // given up: let the products in flight end before tensor memory is freed
             umma_commit(&drained);
-            for (int i = 0; i < (1 << 20) && !gemvq8::mbar_test_wait(&drained, 0); ++i) {}
+#pragma unroll 1
+            for (int k = 0; k < 16; ++k) land(&drained, 0);
         }
         __syncwarp();
     } else {
         const int w = warp < 6 ? 0 : 1, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        auto wait = [&](uint64_t* bar, int phase) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, &abort_flag, p.status)); };
         bool ok = true;
         int item = 0, at = 0;
         for (Walk wk(x.pl, blockIdx.x, p.G, items); wk.more() && ok; wk.next(), ++item) {
@@ -246,40 +276,36 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
             float sum = 0.f;
             for (int n = wk.n0; n < wk.n1 && ok; ++n, ++at) {
                 if ((at & 1) != w) continue;
-                const int s = at % kStagesQ, t = at & 3;
-                ok = wait(&q_full[s], at / kStagesQ) && wait(&s_full[t], at / 4);
+                const int s = at % kStagesL, t = at & 3;
+                ok = wait(&l_full[s], at / kStagesL) && wait(&s_full[t], at / 4);
                 if (!ok) break;
                 tc_fence_after();
                 const int t0 = (wk.it.count + n) * x.tq, r0 = q.old() + t0, r1 = r0 + x.tq - 1;
                 // every query sees every row of the tile
                 const bool whole = t0 + x.tq <= q.n && j0 + kTileK - 1 <= r0 && (a.window == 0 || j0 > r1 - a.window || j0 + kTileK <= a.first);
+                // the queries that see row j are a run of the tile's columns: those from its own token on, as far as the window reaches
+                const int from = clamp_int(j - r0, 0, x.tq) * x.group;
+                const int last = a.window > 0 && j >= a.first ? clamp_int(j + a.window - r0, 0, x.tq) : x.tq, upto = min(last, q.n - t0) * x.group;
                 float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    float z[32];
-                    tmem_ld_32x32(tmem + 128 * t + 32 * q4 + lanes, z);
-                    const float4* ls = reinterpret_cast<const float4*>(&lse[s][32 * q4]);
-                    if (!whole) {            // a weight of 0 for what is not seen
-                        const int4* rs = reinterpret_cast<const int4*>(&rows[s][32 * q4]);
-                        auto hide = [&](float& score, int row) {
-                            if (j > row || (a.window > 0 && j <= row - a.window && j >= a.first)) score = -INFINITY;
-                        };
+                for (int half = 0; half < 2; ++half) {
+                    float z[64];
+                    tmem_ld_32x64(tmem + 128 * t + 64 * half + lanes, z);
+                    const float4* ls = reinterpret_cast<const float4*>(&lse[s][64 * half]);
+                    if (!whole) {
+                        asm volatile("" ::: "memory");          // a branch, not 64 predicated selections in every tile
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const int4 at4 = rs[c];
-                            hide(z[4 * c], at4.x);
-                            hide(z[4 * c + 1], at4.y);
-                            hide(z[4 * c + 2], at4.z);
-                            hide(z[4 * c + 3], at4.w);
-                        }
+                        for (int c = 0; c < 64; ++c)
+                            if (c < from - 64 * half || c >= upto - 64 * half) z[c] = -INFINITY;
                     }
                     const float2 c2 = make_float2(a.c, a.c);
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
+                    for (int c = 0; c < 16; ++c) {
                         const float4 v = ls[c];
-                        const float2 x0 = fma2(make_float2(z[4 * c], z[4 * c + 1]), c2, make_float2(-v.x, -v.y)), x1 = fma2(make_float2(z[4 * c + 2], z[4 * c + 3]), c2, make_float2(-v.z, -v.w));
+                        const float2 x0 = fma2(make_float2(z[4 * c], z[4 * c + 1]), c2, make_float2(v.x, v.y)), x1 = fma2(make_float2(z[4 * c + 2], z[4 * c + 3]), c2, make_float2(v.z, v.w));
                         add[0] = add2(add[0], make_float2(ex2(x0.x), ex2(x0.y)));
-                        add[1] = add2(add[1], make_float2(ex2(x1.x), ex2(x1.y)));
+                        // every fourth pair on the FMA pipe, which takes that off the exponential unit
+                        add[1] = add2(add[1], c & 1 ? ex2_fma(x1) : make_float2(ex2(x1.x), ex2(x1.y)));
                     }
                 }
                 tc_fence_before();
@@ -288,7 +314,7 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&s_empty[t]);
-                    mbar_arrive(&q_empty[s]);
+                    mbar_arrive(&l_empty[s]);
                 }
             }
             if (!ok) break;
