@@ -345,6 +345,113 @@ def test_a_run_of_the_graph(dev, dt):
     serve(dev, dt, step, evict)
 
 
+@pytest.mark.parametrize("dt", [F16, F32])
+def test_rotary_axes_of_the_graph(dev, dt):
+    """Positions per token through the lazy graph, into a paged cache."""
+    g = rng(6)
+    T, G, D = 7, 2, 32
+    f = 10000.0 ** (-np.arange(16) / 16)
+    hi = f.astype(np.float32)
+    at = g.integers(0, 5000, (2, T)).astype(np.int32)
+    h, v = pp.encode(g.standard_normal((T, 5 + G * D)), dt)
+    leaf = lambda a: Tensor.from_data(a, device=dev)  # noqa: E731
+    got = leaf(h).rotary_axes(G, D, leaf(np.stack([hi, (f - hi).astype(np.float32)])), leaf(at), (6, 10), magnitude=0.5, col=5, halves=True)
+    assert got.shape() == (T, G, D)
+    want = pp.rotary(v[:, 5:].reshape(T, G, D), f, at, (6, 10), 0.5, 0, True)
+    assert np.all(np.abs(got.to_numpy() - want) <= HALF_STEP[dt] * np.abs(want) + 1e-6)
+
+
+@pytest.mark.parametrize("dt,new", [(F16, [1, 1, 1]), (BF16, [40, 3, 70]), (F32, [2, 5, 1])])
+def test_a_captured_step_replayed_over_new_lengths(dt, new):
+    """Append, attention with sums and eviction in one CUDA graph: replayed after the host has moved lengths, starts and rows on."""
+    import torch
+    from ratchet_b200 import Device
+    stream = torch.cuda.Stream()
+    d = Device(0, stream=stream.cuda_stream)
+    g = rng(13)
+    H, G, D, R, MP, T = 4, 2, 64, 16, 16, sum(new)
+    table = up(d, g.permutation(3 * MP).reshape(3, MP).astype(np.int32))
+    keys, values, mass = d.zeros(dt, (3 * MP, G, R, D)), d.zeros(dt, (3 * MP, G, R, D)), d.zeros(F32, (3, G, MP * R))
+    starts, lengths, cut = up(d, np.zeros(4, np.int32)), up(d, np.zeros(3, np.int32)), d.zeros(capi.I32, (3,))
+    rows = {n: d.zeros(dt, (T, w * D)) for n, w in (("q", H), ("k", G), ("v", G))}
+    c = PagedCache(keys, values, table, lengths, starts, mass)
+    into = PagedCache(keys, values, table, cut, mass=mass)
+    q, out = rows["q"].view((T, H, D)), d.zeros(dt, (T, H * D))
+    scratch = d.empty(F32, (max(4, d.paged_attention_scratch(q, c) // 4),))
+    cutting = d.empty(F32, (max(4, d.paged_evict_scratch(c, 150) // 4),))
+
+    def step():
+        d.paged_append(rows["k"], rows["v"], c)
+        d.paged_attention(q, c, 0.125, scratch=scratch, out=out)
+        d.paged_evict(c, into, 150, 2, 100, scratch=cutting)
+
+    step()                                                  # attributes are set once outside the capture
+    d.sync()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+        with pytest.raises(RatchetCudaError):               # scratch from the pool would belong to others by the time of a replay
+            d.paged_attention(q, c, 0.125, out=out)
+    k64, v64, have, m64 = [np.zeros((0, G, D))] * 3, [np.zeros((0, G, D))] * 3, [0] * 3, [np.zeros((G, 0))] * 3
+    for turn in range(4):
+        order = new if turn % 2 == 0 else new[::-1]         # other lengths than those captured
+        host = {n: pp.encode(g.standard_normal((T, b.shape[1])), dt) for n, b in rows.items()}
+        for n, b in rows.items():
+            d.h2d(b.ptr, host[n][0])
+        ref = pp.Cache.__new__(pp.Cache)
+        ref.dt, ref.new, ref.G, ref.D, ref.E, ref.R = dt, order, G, D, D, R
+        ref.starts = np.concatenate([[0], np.cumsum(order)]).astype(np.int32)
+        for s, n in enumerate(order):
+            t = ref.starts[s]
+            k64[s] = np.concatenate([k64[s], host["k"][1][t:t + n].reshape(n, G, D)])
+            v64[s] = np.concatenate([v64[s], host["v"][1][t:t + n].reshape(n, G, D)])
+            m64[s] = np.concatenate([m64[s], np.zeros((G, n))], 1)
+        ref.k, ref.v, ref.lengths = k64, v64, [len(x) for x in k64]
+        d.h2d(starts.ptr, ref.starts)
+        d.h2d(lengths.ptr, np.asarray(ref.lengths, np.int32))
+        d.sync()
+        graph.replay()
+        torch.cuda.synchronize()
+        want, size, grown = pp.attention(ref, host["q"][1].reshape(T, H, D), 0.125)
+        assert close(get(out).reshape(T, H, D), want, size, dt, 5.0), turn
+        m64 = [a + b for a, b in zip(m64, grown)]
+        sums = mass.to_numpy()
+        assert np.array_equal(cut.to_numpy(), np.minimum(ref.lengths, 150))
+        for s, L in enumerate(ref.lengths):
+            kept = [pp.kept(m64[s][h], L, 150, 2, 100) for h in range(G)]
+            k64[s] = np.stack([k64[s][kept[h], h] for h in range(G)], 1)
+            v64[s] = np.stack([v64[s][kept[h], h] for h in range(G)], 1)
+            m64[s] = np.stack([m64[s][h, kept[h]] for h in range(G)])
+            assert np.allclose(sums[s, :, :len(kept[0])], m64[s], rtol=1e-4, atol=1e-6)
+    del graph
+    d.sync()
+    d.close()
+
+
+def test_two_handles_at_once(dev):
+    """Calls on two streams of one device at the same time, each with its pool's scratch."""
+    from ratchet_b200 import Device
+    other = Device(0)
+    g = rng(17)
+    jobs = []
+    for d, new, lengths, dt in ((dev, [1] * 6, [700] * 6, F16), (other, [200, 1], [900, 300], BF16)):
+        c = pp.Cache(g, dt, new, lengths, 2, 64, 64, 32)
+        q, qv = put(d, g.standard_normal((sum(new), 8, 64)), dt)
+        jobs.append((d, c, device_cache(d, c, np.zeros((len(new), 2, c.rows))), q, qv, dt))
+    outs = [[j[0].paged_attention(j[3], j[2], 0.125) for j in jobs] for _ in range(6)]
+    for k, (d, c, _, _, qv, dt) in enumerate(jobs):
+        want, size, _ = pp.attention(c, qv, 0.125)
+        for o in outs:
+            assert close(get(o[k]).reshape(want.shape), want, size, dt, 5.0)
+    other.sync()
+    for o in outs:
+        o[1].free()
+    for b in (jobs[1][3], jobs[1][2].keys, jobs[1][2].values, jobs[1][2].table, jobs[1][2].starts, jobs[1][2].lengths, jobs[1][2].mass):
+        b.free()
+    other.close()
+
+
 # ---------------------------------------------------------------------------------------- refusals
 def test_bad_indexes_are_reported(dev):
     g = rng(2)

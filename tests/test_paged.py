@@ -1,0 +1,92 @@
+"""Paged caches where no device is needed: the plain restatement that the GPU tests compare with, against brute force, and what the graph's
+builders refuse."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from . import paged_plain as pp
+from .test_graph_cpu import _leaf
+
+
+def rng(seed):
+    return np.random.Generator(np.random.PCG64(seed))
+
+
+@pytest.mark.parametrize("new,lengths,window,first,sink", [([1, 4], [5, 9], 0, 0, False), ([3, 0, 7], [3, 2, 20], 4, 2, True), ([6], [6], 1, 0, True), ([2], [11], 3, 20, False)])
+def test_plain_attention_by_brute_force(new, lengths, window, first, sink):
+    g = rng(sum(lengths))
+    c = pp.Cache(g, pp.F32, new, lengths, 2, 8, 8, 16)
+    q = g.standard_normal((sum(new), 4, 8))
+    sk = g.standard_normal(4) if sink else None
+    out, _, mass = pp.attention(c, q, 0.3, sk, window, first)
+    for s, (n, L) in enumerate(zip(new, lengths)):
+        got = np.zeros((2, L))
+        for i in range(n):
+            r = L - n + i
+            for h in range(4):
+                rows = [j for j in range(r + 1) if not window or j > r - window or j < first]
+                e = [np.exp(0.3 * q[c.starts[s] + i, h] @ c.k[s][j, h // 2]) for j in rows]
+                total = sum(e) + (np.exp(sk[h]) if sink else 0)
+                assert np.allclose(out[c.starts[s] + i, h], sum(x * c.v[s][j, h // 2] for x, j in zip(e, rows)) / total)
+                for x, j in zip(e, rows):
+                    got[h // 2, j] += x / total
+        assert np.allclose(got, mass[s])
+
+
+def test_plain_eviction_keeps_the_heaviest_and_the_lower_of_equal_ones():
+    m = np.array([9, 1, 5, 5, np.nan, 5, 0, -np.inf, np.inf, 2, 3], np.float32)
+    assert list(pp.kept(m, 11, 5, 1, 1)) == [0, 2, 3, 8, 10]
+    assert list(pp.kept(m, 11, 11, 1, 1)) == list(range(11))
+    assert list(pp.kept(m, 11, 10, 0, 0)) == [0, 1, 2, 3, 5, 6, 7, 8, 9, 10]
+    assert list(pp.kept(m, 11, 3, 1, 2)) == [0, 9, 10]
+
+
+def test_pages_hold_the_rows_and_nothing_else():
+    c = pp.Cache(rng(1), pp.BF16, [2, 1], [33, 16], 2, 8, 16, 16)
+    assert c.table.shape == (2, 3) and list(c.table[1, 1:]) == [-1, -1]
+    assert np.array_equal(c.rows_of(c.keys, c.table, 0, 33), c.k[0]) and np.array_equal(c.rows_of(c.values, c.table, 1, 16), c.v[1])
+    assert np.isnan(pp.decode(c.keys, c.dt)).sum() == (len(c.keys) * 16 - 49) * 2 * 8
+
+
+def test_builders_refuse_what_does_not_fit():
+    from ratchet_b200 import capi
+    lib, F16, I32, F32 = capi.lib(), capi.F16, capi.I32, capi.F32
+    leaf = lambda dt, *shape: _leaf(lib, capi, shape, dt)  # noqa: E731
+    keys, values, table, starts, lengths = leaf(F16, 4, 2, 16, 64), leaf(F16, 4, 2, 16, 32), leaf(I32, 3, 2), leaf(I32, 4), leaf(I32, 3)
+    mass, k, v, q = leaf(F32, 3, 2, 32), leaf(F16, 5, 130), leaf(F16, 5, 64), leaf(F16, 5, 4, 64)
+    out = C.c_void_p()
+    ref = C.byref(out)
+
+    def shape():
+        t = capi.rcu_tensor()
+        lib.rcu_lazy_info(out, C.byref(t))
+        got = t.dt, tuple(t.shape[i] for i in range(t.rank))
+        lib.rcu_lazy_release(out)
+        return got
+
+    assert lib.rcu_lazy_paged_append(k, 2, v, 0, keys, values, table, starts, lengths, mass, ref) == capi.OK and shape() == (I32, (3,))
+    assert lib.rcu_lazy_paged_append(k, 3, v, 0, keys, values, table, starts, lengths, None, ref) == capi.ERR_INVALID_ARG          # past the rows' end
+    assert lib.rcu_lazy_paged_append(k, 0, q, 0, keys, values, table, starts, lengths, None, ref) == capi.ERR_INVALID_ARG
+    assert lib.rcu_lazy_paged_append(k, 0, v, 0, keys, values, table, starts, starts, None, ref) == capi.ERR_INVALID_ARG           # four lengths of three sequences
+    assert lib.rcu_lazy_paged_attention(q, keys, values, table, starts, lengths, None, None, 0, 0, 0.1, ref) == capi.OK and shape() == (F16, (5, 128))
+    assert lib.rcu_lazy_paged_attention(q, values, values, table, starts, lengths, None, None, 0, 0, 0.1, ref) == capi.ERR_INVALID_ARG
+    assert lib.rcu_lazy_paged_attention(None, keys, values, table, starts, lengths, None, None, 0, 0, 0.1, ref) == capi.ERR_INVALID_ARG
+    # pages that a node of the graph is still to make
+    made = C.c_void_p()
+    assert lib.rcu_lazy_unary(8, keys, C.byref(made)) == capi.OK
+    assert lib.rcu_lazy_paged_attention(q, made, values, table, starts, lengths, None, None, 0, 0, 0.1, ref) == capi.ERR_INVALID_ARG
+    into = (keys, values, table, mass)
+    assert lib.rcu_lazy_paged_evict(keys, values, table, lengths, mass, *into, 8, 2, 6, ref) == capi.OK and shape() == (I32, (3,))
+    assert lib.rcu_lazy_paged_evict(keys, values, table, lengths, mass, *into, 8, 2, 7, ref) == capi.ERR_INVALID_ARG
+    assert lib.rcu_lazy_paged_evict(keys, values, table, lengths, mass, *into, 0, 0, 0, ref) == capi.ERR_INVALID_ARG
+    assert lib.rcu_lazy_paged_evict(keys, values, table, lengths, None, *into, 8, 2, 6, ref) == capi.ERR_INVALID_ARG
+    freqs, at, x = leaf(F32, 2, 16), leaf(I32, 2, 5), leaf(F16, 5, 130)
+    sec = lambda *s: (C.c_uint32 * len(s))(*s)  # noqa: E731
+    axes = lambda col, heads, dim, first, positions, s: lib.rcu_lazy_rotary_axes(x, col, heads, dim, first, freqs, 1.0, positions, s, 0, ref)  # noqa: E731
+    assert axes(2, 2, 64, 32, at, sec(10, 6)) == capi.OK and shape() == (F16, (5, 2, 64))
+    assert axes(3, 2, 64, 32, at, sec(10, 6)) == capi.ERR_INVALID_ARG                  # past the rows' end
+    assert axes(2, 2, 64, 33, at, sec(10, 6)) == capi.ERR_INVALID_ARG                  # past the head's
+    assert axes(2, 2, 64, 0, at, sec(10, 5)) == capi.ERR_INVALID_ARG                   # a pair without an axis
+    assert axes(2, 2, 64, 0, leaf(F32, 2, 5), sec(10, 6)) == capi.ERR_INVALID_ARG
+    assert axes(2, 2, 64, 0, leaf(I32, 2, 4), sec(10, 6)) == capi.ERR_INVALID_ARG
