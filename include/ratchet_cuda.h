@@ -322,8 +322,9 @@ rcu_status rcu_paged_append(rcu_device* dev, const rcu_tensor* k, uint32_t k_col
  * h / (H / kv_heads).  The token at row r of its sequence sees rows j <= r, with window > 0 only those with j > r - window or j < first.
  * sink F32 [H] (nullable): exp(sink[h]) joins the denominator.  dst [tokens, H * vdim].  Where mass is kept, every row's sum grows by the
  * weights (shares of the denominator) that the group's heads and the new tokens give it; sums are formed in the same order in every call.
- * scratch (nullable): device memory of rcu_paged_attention_scratch bytes, any dtype; NULL takes it from the pool, which is refused while the
- * stream is being captured.  Calls that share a scratch must not overlap. */
+ * dst must not overlap q.  With mass, sequences * kv_heads are 65535 at most.
+ * scratch (nullable): device memory of rcu_paged_attention_scratch bytes on a 256-byte boundary, any dtype; NULL takes it from the pool, which is
+ * refused while the stream is being captured.  Calls that share a scratch must not overlap. */
 rcu_status rcu_paged_attention(rcu_device* dev, const rcu_tensor* q, const rcu_paged* cache, const rcu_tensor* sink, uint32_t window, uint32_t first,
                                float scale, const rcu_tensor* scratch, rcu_tensor* dst);
 uint64_t rcu_paged_attention_scratch(rcu_device* dev, const rcu_tensor* q, const rcu_paged* cache);

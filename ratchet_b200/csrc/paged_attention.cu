@@ -112,14 +112,19 @@ rcu_status rcu_paged_attention(rcu_device* dev, const rcu_tensor* q, const rcu_p
     RCU_REQUIRE(dev, H >= 1 && H % p.G == 0 && H <= 65535, "paged_attention: %llu query heads over %d kv heads", (unsigned long long)H, p.G);
     RCU_REQUIRE(dev, !sink || (sink->dt == RCU_F32 && t_numel(sink) == H), "paged_attention: one f32 sink per query head");
     RCU_REQUIRE(dev, t_numel(dst) == T * H * p.E, "paged_attention: dst holds %llu elements, expected %llu", (unsigned long long)t_numel(dst), (unsigned long long)(T * H * p.E));
-    RCU_REQUIRE(dev, T * H < (1ull << 31) && (uint64_t)p.S * p.G <= 65535, "paged_attention: %llu tokens of %llu heads, %d sequences", (unsigned long long)T, (unsigned long long)H, p.S);
+    RCU_REQUIRE(dev, T * H < (1ull << 31) && (!p.mass || (uint64_t)p.S * p.G <= 65535), "paged_attention: %llu tokens of %llu heads, %d sequences", (unsigned long long)T,
+                (unsigned long long)H, p.S);
+    const size_t e = dt_esize(q->dt);
+    const char *qb = (const char*)q->data, *ob = (const char*)dst->data;
+    RCU_REQUIRE(dev, ob >= qb + T * H * p.D * e || qb >= ob + T * H * p.E * e, "paged_attention: the output overlaps the queries");
     if (T == 0) return RCU_OK;
     a.q = q->data;
     a.out = dst->data;
     a.sink = sink ? (const float*)sink->data : nullptr;
     a.H = (int)H;
-    a.window = window > (1u << 30) ? 0 : (int)window;
-    a.first = first > (1u << 30) ? 1 << 30 : (int)first;
+    // a window as long as a sequence's room is none; sums of rows and windows stay below 2^31
+    a.window = window >= (uint64_t)p.MP << p.shift ? 0 : (int)window;
+    a.first = first > (1u << 29) ? 1 << 29 : (int)first;
     a.c = scale * kLog2e;
     DevGuard guard(dev->ordinal);
     Scratch mem(dev);

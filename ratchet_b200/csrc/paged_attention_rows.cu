@@ -353,7 +353,11 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             const int j = slice_at(i);
             if (j >= end) continue;
             const int st = had % kRing;
-            if (ok) ok = wait_warp(&full[warp][st], had / kRing, &abort_flag, p.status);
+            if (ok) {
+                ok = wait_warp(&full[warp][st], had / kRing, &abort_flag, p.status);
+                if (!ok)                   // given up: let the copies in flight land before the memory is somebody else's
+                    for (int k = had; k < asked; ++k) land(&full[warp][k % kRing], k / kRing);
+            }
             ++had;
             if (!ok) continue;
             unsigned char *ks = ring + st * slot_bytes, *vs = ks + kbytes;
@@ -374,8 +378,6 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             else part.step(x, smem_u32(ks), smem_u32(vs), masked, j, pos[0], pos[1], to[0], to[1], nullptr);
             __syncwarp();
         }
-        if (!ok)                           // given up: let the copies in flight land before the memory is somebody else's
-            for (; had < asked; ++had) land(&full[warp][had % kRing], had / kRing);
         // the warps' maxima and sums
         __syncthreads();
         float* sums = reinterpret_cast<float*>(base);

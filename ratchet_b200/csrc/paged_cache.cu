@@ -22,10 +22,10 @@ rcu_status view(rcu_device* dev, const char* op, const rcu_paged* c, uint64_t to
     RCU_REQUIRE(dev, ((reinterpret_cast<uintptr_t>(k.data) | reinterpret_cast<uintptr_t>(v.data)) & 15) == 0, "%s: pages start on 16 bytes", op);
     RCU_REQUIRE(dev, c->table.dt == RCU_I32 && c->table.rank == 2 && c->lengths.dt == RCU_I32, "%s: the table is i32 [sequences, max_pages], lengths are i32", op);
     const uint64_t S = c->table.shape[0], MP = c->table.shape[1];
-    RCU_REQUIRE(dev, S >= 1 && S <= (1u << 20) && MP >= 1 && MP * R <= (1ull << 30), "%s: %llu sequences of up to %llu pages", op, (unsigned long long)S, (unsigned long long)MP);
+    RCU_REQUIRE(dev, S >= 1 && S <= (1u << 20) && MP >= 1 && MP * R <= (1ull << 29), "%s: %llu sequences of up to %llu pages", op, (unsigned long long)S, (unsigned long long)MP);
     RCU_REQUIRE(dev, t_numel(&c->lengths) == S, "%s: one length per sequence", op);
     if (starts) RCU_REQUIRE(dev, c->starts.dt == RCU_I32 && t_numel(&c->starts) == S + 1, "%s: starts are i32 [sequences + 1]", op);
-    RCU_REQUIRE(dev, tokens < (1ull << 30), "%s: %llu tokens", op, (unsigned long long)tokens);
+    RCU_REQUIRE(dev, tokens <= (1ull << 29), "%s: %llu tokens", op, (unsigned long long)tokens);
     const bool mass = c->mass.data != nullptr;
     if (mass)
         RCU_REQUIRE(dev, c->mass.dt == RCU_F32 && c->mass.rank == 3 && c->mass.shape[0] == S && c->mass.shape[1] == G && c->mass.shape[2] == MP * R,

@@ -263,6 +263,41 @@ def test_evict(dev, dt, place, lengths, G, D, E, R, keep, first, recent):
 
 
 # ---------------------------------------------------------------------------------------- together
+@pytest.mark.parametrize("dt,new", [(BF16, [1, 2]), (F16, [90, 40]), (F32, [3, 1])])
+def test_pages_beyond_32_bits(dev, dt, new):
+    """Pools of more than 2^32 bytes: rows written to, read from and moved between pages at both ends."""
+    g = rng(23)
+    G, D, R, lengths = 4, 128, 256, [300, 520]
+    pages = 2 ** 32 // (G * R * D * (4 if dt == F32 else 2)) + 9
+    keys, values = dev.empty(dt, (pages, G, R, D)), dev.empty(dt, (pages, G, R, D))
+    table = np.array([[pages - 1, 3, 0], [1, pages - 2, pages - 5]], np.int32)
+    c = pp.Cache(g, dt, lengths, lengths, G, D, D, R)
+    k, _ = put(dev, np.concatenate([x.reshape(-1, G * D) for x in c.k]), dt)
+    v, _ = put(dev, np.concatenate([x.reshape(-1, G * D) for x in c.v]), dt)
+    ints = lambda a: up(dev, np.asarray(a, np.int32))  # noqa: E731
+    mass = up(dev, g.random((2, G, 3 * R)).astype(np.float32))
+    cache = PagedCache(keys, values, ints(table), ints(lengths), ints([0, 300, 820]), mass)
+    before = mass.to_numpy()
+    dev.paged_append(k, v, cache)
+    assert np.all(mass.to_numpy()[0, :, :300] == 0) and np.array_equal(mass.to_numpy()[0, :, 300:], before[0, :, 300:])
+    c.new, c.starts = new, np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    q, qv = put(dev, g.standard_normal((sum(new), 8, D)), dt)
+    want, size, sums = pp.attention(c, qv, 0.09)
+    now = PagedCache(keys, values, cache.table, cache.lengths, ints(c.starts), mass)
+    assert close(get(dev.paged_attention(q, now, 0.09)).reshape(want.shape), want, size, dt, 5.0)
+    grown = mass.to_numpy()
+    into = PagedCache(keys, values, ints([[pages - 7], [5]]), dev.zeros(capi.I32, (2,)), mass=dev.zeros(F32, (2, G, R)))
+    dev.paged_evict(now, into, 200, 3, 50)
+    one = dev.wrap(dt, (1, G, R, D), keys.ptr + (pages - 7) * G * R * D * (4 if dt == F32 else 2))
+    got = get(one)[0]
+    for h in range(G):
+        assert np.allclose(grown[0, h, :300], sums[0][h], rtol=1e-4, atol=1e-6)
+        assert np.array_equal(got[h, :200], c.k[0][pp.kept(grown[0, h], 300, 200, 3, 50), h])
+    keys.free()
+    values.free()
+    dev.check(dev._lib.rcu_pool_trim(dev.handle))
+
+
 def serve(dev, dt, step, evict):
     """Three sequences: prompts, then single tokens, their rows cut to 40 whenever one has more than 60; against float64 all the way."""
     g = rng(8)
@@ -525,7 +560,8 @@ def test_refusals(dev):
         lambda: dev.rotary_axes(x, 2, 64, fr, at, (32,), out=dev.wrap(F16, (3, 2, 64), x.ptr)),
     ]
     m = cache(mass=True)
-    bad += [lambda: dev.paged_evict(m, m, 8), lambda: dev.paged_evict(m, PagedCache(m.keys, m.values, m.table, m.lengths, mass=m.mass), 8),
+    bad += [lambda: dev.paged_attention(q, cache(), 0.1, out=q.view((3, 256))),
+            lambda: dev.paged_evict(m, m, 8), lambda: dev.paged_evict(m, PagedCache(m.keys, m.values, m.table, m.lengths, mass=m.mass), 8),
             lambda: dev.paged_evict(m, PagedCache(m.values, m.keys, m.table, z(I32, 2), mass=m.mass), 8)]
     for f in bad:
         with pytest.raises(RatchetCudaError):
