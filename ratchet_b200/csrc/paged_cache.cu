@@ -74,6 +74,17 @@ __global__ void __launch_bounds__(128) append_kernel(const View p, const Unit* _
         }
         if (p.T == 0) return;
     }
+    // the row's first units are on their way while its place is found
+    const Unit *ks = k + t * k_pitch, *vs = v + t * v_pitch;
+    constexpr int kAhead = 2;
+    const int kn = p.G * du, vn = p.G * eu;
+    Unit kb[kAhead], vb[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+        const int i = threadIdx.x + 128 * j;
+        if (i < kn) kb[j] = ks[i];
+        if (i < vn) vb[j] = vs[i];
+    }
     const int s = seq_of_token(p, t);
     if (s < 0) return;
     const Seq q = seq_of(p, s);
@@ -82,11 +93,17 @@ __global__ void __launch_bounds__(128) append_kernel(const View p, const Unit* _
     const int page = page_of(p, s, r), at = r & (p.R - 1);
     Unit* kd = const_cast<Unit*>(reinterpret_cast<const Unit*>(p.keys)) + ((size_t)page * p.G * p.R + at) * du;
     Unit* vd = const_cast<Unit*>(reinterpret_cast<const Unit*>(p.values)) + ((size_t)page * p.G * p.R + at) * eu;
-    const Unit *ks = k + t * k_pitch, *vs = v + t * v_pitch;
+    auto put = [&](Unit* to, int i, int units, const Unit& value) { to[(size_t)(i / units) * p.R * units + i % units] = value; };
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+        const int i = threadIdx.x + 128 * j;
+        if (i < kn) put(kd, i, du, kb[j]);
+        if (i < vn) put(vd, i, eu, vb[j]);
+    }
 #pragma unroll 4
-    for (int i = threadIdx.x; i < p.G * du; i += 128) kd[(size_t)(i / du) * p.R * du + i % du] = ks[i];
+    for (int i = threadIdx.x + 128 * kAhead; i < kn; i += 128) put(kd, i, du, ks[i]);
 #pragma unroll 4
-    for (int i = threadIdx.x; i < p.G * eu; i += 128) vd[(size_t)(i / eu) * p.R * eu + i % eu] = vs[i];
+    for (int i = threadIdx.x + 128 * kAhead; i < vn; i += 128) put(vd, i, eu, vs[i]);
     if (p.mass)
         for (int g = threadIdx.x; g < p.G; g += 128) p.mass[((size_t)s * p.G + g) * ((size_t)p.MP << p.shift) + r] = 0.f;
 }

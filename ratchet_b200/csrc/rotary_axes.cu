@@ -45,47 +45,57 @@ __global__ void __launch_bounds__(256) rotary_axes_kernel(const AxesArgs a, cons
     if constexpr (VEC) {
         constexpr int V = 16 / (int)sizeof(T);
         struct alignas(16) Vec { T v[V]; };
+        // a thread has one place of a row, in every token or every few, and asks for several tokens at once
+        const int places = a.H * (a.halves ? a.pairs / V + (a.D - 2 * a.pairs) / V : a.D / V), abreast = max(1, 256 / places);
+        const int first_place = places < 256 ? (int)threadIdx.x % places : (int)threadIdx.x, first_token = places < 256 ? (int)threadIdx.x / places : 0;
+        if (first_token >= abreast) return;
         if (a.halves) {
             // units of V pairs: V features of the first half and V of the second; then what is not turned
             const int units = a.pairs / V, rest = (a.D - 2 * a.pairs) / V, per = units + rest;
-            for (int j = threadIdx.x; j < n * a.H * per; j += 256) {
-                const int t = j / (a.H * per), h = j / per % a.H, u = j % per;
-                const T* xr = x + (t0 + t) * a.pitch + (size_t)h * a.D;
-                T* o = out + ((t0 + t) * a.H + h) * (size_t)a.D;
-                if (u >= units) {
-                    int d = (u - units) * V;
-                    if (d >= lo) d += 2 * a.pairs;
-                    *reinterpret_cast<Vec*>(o + d) = *reinterpret_cast<const Vec*>(xr + d);
-                    continue;
-                }
-                const int d = lo + u * V;
-                const Vec p = *reinterpret_cast<const Vec*>(xr + d), q = *reinterpret_cast<const Vec*>(xr + d + a.pairs);
-                Vec y, z;
+            for (int j = first_place; j < places; j += 256) {
+                const int h = j / per, u = j - h * per;
+                int d = u < units ? lo + u * V : (u - units) * V;
+                if (u >= units && d >= lo) d += 2 * a.pairs;
+                const int e = u < units ? d + a.pairs : d;
+                const T* xr = x + t0 * a.pitch + (size_t)h * a.D;
+                T* o = out + (t0 * a.H + h) * (size_t)a.D;
+#pragma unroll 4
+                for (int t = first_token; t < n; t += abreast) {
+                    Vec p = *reinterpret_cast<const Vec*>(xr + t * a.pitch + d), q = *reinterpret_cast<const Vec*>(xr + t * a.pitch + e);
+                    if (u < units) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float2 w = cs[t * a.pairs + u * V + e];
-                    const float f = to_f32<T>(p.v[e]), g = to_f32<T>(q.v[e]);
-                    y.v[e] = from_f32<T>(f * w.x - g * w.y);
-                    z.v[e] = from_f32<T>(g * w.x + f * w.y);
+                        for (int i = 0; i < V; ++i) {
+                            const float2 w = cs[t * a.pairs + u * V + i];
+                            const float f = to_f32<T>(p.v[i]), g = to_f32<T>(q.v[i]);
+                            p.v[i] = from_f32<T>(f * w.x - g * w.y);
+                            q.v[i] = from_f32<T>(g * w.x + f * w.y);
+                        }
+                        *reinterpret_cast<Vec*>(o + (size_t)t * a.H * a.D + e) = q;
+                    }
+                    *reinterpret_cast<Vec*>(o + (size_t)t * a.H * a.D + d) = p;
                 }
-                *reinterpret_cast<Vec*>(o + d) = y;
-                *reinterpret_cast<Vec*>(o + d + a.pairs) = z;
             }
         } else {
             const int per = a.D / V;
-            for (int j = threadIdx.x; j < n * a.H * per; j += 256) {
-                const int t = j / (a.H * per), h = j / per % a.H, d = j % per * V;
-                Vec p = *reinterpret_cast<const Vec*>(x + (t0 + t) * a.pitch + (size_t)h * a.D + d);
-                if (d >= lo && d < hi) {
+            for (int j = first_place; j < places; j += 256) {
+                const int h = j / per, d = (j - h * per) * V;
+                const T* xr = x + t0 * a.pitch + (size_t)h * a.D + d;
+                T* o = out + (t0 * a.H + h) * (size_t)a.D + d;
+                const bool turned = d >= lo && d < hi;
+#pragma unroll 4
+                for (int t = first_token; t < n; t += abreast) {
+                    Vec p = *reinterpret_cast<const Vec*>(xr + t * a.pitch);
+                    if (turned) {
 #pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        const float2 w = cs[t * a.pairs + (d - lo + e) / 2];
-                        const float f = to_f32<T>(p.v[e]), g = to_f32<T>(p.v[e + 1]);
-                        p.v[e] = from_f32<T>(f * w.x - g * w.y);
-                        p.v[e + 1] = from_f32<T>(g * w.x + f * w.y);
+                        for (int e = 0; e < V; e += 2) {
+                            const float2 w = cs[t * a.pairs + (d - lo + e) / 2];
+                            const float f = to_f32<T>(p.v[e]), g = to_f32<T>(p.v[e + 1]);
+                            p.v[e] = from_f32<T>(f * w.x - g * w.y);
+                            p.v[e + 1] = from_f32<T>(g * w.x + f * w.y);
+                        }
                     }
+                    *reinterpret_cast<Vec*>(o + (size_t)t * a.H * a.D) = p;
                 }
-                *reinterpret_cast<Vec*>(out + ((t0 + t) * a.H + h) * (size_t)a.D + d) = p;
             }
         }
     } else {
