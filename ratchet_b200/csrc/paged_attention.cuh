@@ -50,8 +50,6 @@ struct Plan {
 };
 
 #ifdef __CUDACC__
-struct Span;
-__device__ __forceinline__ Span span_of(int window, int first, int r0, int r1);
 // Tiles that tokens at rows r0 .. r1 see: the first `head` ones, then lo, lo + 1, ..
 struct Span {
     int head, lo, count;

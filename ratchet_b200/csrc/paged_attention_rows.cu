@@ -15,7 +15,7 @@
 namespace paged {
 namespace {
 
-constexpr int kSlice = 16, kRing = 3, kPlanned = 256;
+constexpr int kSlice = 16, W = 8, kPlanned = 256;          // rows of a slice; warps of a CTA; items that every CTA works out for itself
 
 template <class T> struct Form {
     static constexpr int kRows = 16, kCols = 64;          // columns of 128 bytes
@@ -62,7 +62,7 @@ template <class T> struct Part {
     uint32_t q[8][4];
     float o[16][4], m[2], l[2];
 
-    __device__ __forceinline__ void begin(const RowsArgs& x, const T* q0, const T* q1, float*, int) {      // the lane's two rows, nullable
+    __device__ __forceinline__ void begin(const RowsArgs& x, const T* q0, const T* q1) {      // the lane's two rows, nullable
         const int lane = threadIdx.x & 31;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -80,7 +80,7 @@ template <class T> struct Part {
         l[0] = l[1] = 0.f;
     }
     // scores z of the slice's keys 8 t + 2 (lane % 4) + e: z[t][e] row lane / 4, z[t][2 + e] row lane / 4 + 8
-    __device__ __forceinline__ void step(const RowsArgs& x, uint32_t ks, uint32_t vs, bool masked, int j, int pos0, int pos1, float* to0, float* to1, float*) {
+    __device__ __forceinline__ void step(const RowsArgs& x, uint32_t ks, uint32_t vs, bool masked, int j, int pos0, int pos1, float* to0, float* to1) {
         const int lane = threadIdx.x & 31;
         const AttendArgs& a = x.a;
         float z[2][4] = {};
@@ -168,7 +168,7 @@ template <> struct Part<float> {
     float4 o[8];
     float m[4], l[4];
 
-    __device__ __forceinline__ void begin(const RowsArgs&, const float*, const float*, float*, int) {
+    __device__ __forceinline__ void begin() {
 #pragma unroll
         for (int r = 0; r < 8; ++r) o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -246,7 +246,7 @@ template <> struct Part<float> {
     }
 };
 
-template <class T, int W>
+template <class T, int kRing>
 __global__ void __launch_bounds__(W * 32, 1)
 rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ RowsArgs x) {
     constexpr int BQ = Form<T>::kRows, C = Form<T>::kCols;
@@ -337,7 +337,7 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
                 pos[r] = u < count ? row_of(u) : -1;
                 if (x.scores && u < count) to[r] = x.scores + query(u) * room;
             }
-            part.begin(x, nullptr, nullptr, nullptr, 0);
+            part.begin();
             __syncthreads();
         } else {
             const int u0 = lane >> 2, u1 = u0 + 8;
@@ -345,7 +345,7 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             pos[1] = u1 < count ? row_of(u1) : -1;
             if (x.scores && u0 < count) to[0] = x.scores + query(u0) * room;
             if (x.scores && u1 < count) to[1] = x.scores + query(u1) * room;
-            part.begin(x, u0 < count ? (const T*)a.q + query(u0) * p.D : nullptr, u1 < count ? (const T*)a.q + query(u1) * p.D : nullptr, nullptr, 0);
+            part.begin(x, u0 < count ? (const T*)a.q + query(u0) * p.D : nullptr, u1 < count ? (const T*)a.q + query(u1) * p.D : nullptr);
         }
 #pragma unroll 1
         for (int i = 0; i < slices; ++i) {
@@ -375,7 +375,7 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
                 __syncwarp();
             }
             if constexpr (f32) part.step(x, ks, vs, masked, j, pos, to, qs, own[warp]);
-            else part.step(x, smem_u32(ks), smem_u32(vs), masked, j, pos[0], pos[1], to[0], to[1], nullptr);
+            else part.step(x, smem_u32(ks), smem_u32(vs), masked, j, pos[0], pos[1], to[0], to[1]);
             __syncwarp();
         }
         // the warps' maxima and sums
@@ -538,13 +538,15 @@ template <class T> rcu_status launch_rows(rcu_device* dev, const AttendArgs& a, 
         const rcu_status st = plan_items(dev, p, x.pl, a.window, a.first, x.group);
         if (st != RCU_OK) return st;
     }
-    // eight warps where their rings fit, which is always in 16 bits
-    const size_t warp_ring = (size_t)kRing * (x.nb + x.eb) * kSlice * 128, warp_sums = (size_t)Form<T>::kRows * p.E * 4;
-    const int warps = 8 * warp_ring <= 192 * 1024 ? 8 : 4;
-    const size_t smem = 1024 + warps * (warp_ring > warp_sums ? warp_ring : warp_sums);
-    void (*kern)(CUtensorMap, CUtensorMap, RowsArgs) = warps == 8 ? rows_kernel<T, 8> : rows_kernel<T, sizeof(T) == 4 ? 4 : 8>;
+    // Rings three slices deep, which always fit in 16 bits; in f32 as deep as shared memory allows: eight warps with a ring of one or two slices are faster than
+    // four with three.
+    const size_t slots = (size_t)W * (x.nb + x.eb) * kSlice * 128, sums = (size_t)W * Form<T>::kRows * p.E * 4;
+    const int ring = 3 * slots <= 192 * 1024 ? 3 : 2 * slots <= 192 * 1024 ? 2 : 1;
+    const size_t smem = 1024 + (ring * slots > sums ? ring * slots : sums);
+    constexpr bool f32 = sizeof(T) == 4;
+    void (*kern)(CUtensorMap, CUtensorMap, RowsArgs) = ring == 3 ? rows_kernel<T, 3> : ring == 2 ? rows_kernel<T, f32 ? 2 : 3> : rows_kernel<T, f32 ? 1 : 3>;
     RCU_CUDA(dev, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    RCU_CUDA(dev, rcu_launch(dev, kern, x.pl.ctas, warps * 32, smem, km, vm, x));
+    RCU_CUDA(dev, rcu_launch(dev, kern, x.pl.ctas, W * 32, smem, km, vm, x));
     RCU_LAUNCH_CHECK(dev);
     if (x.pl.ctas > 1) {
         rcu_launch(dev, rows_merge_kernel<T>, x.pl.ctas - 1, 256, (size_t)x.pl.ctas * Form<T>::kRows * 4, a, x.pl, x.group);
