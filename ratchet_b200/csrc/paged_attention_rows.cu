@@ -7,8 +7,8 @@
 //   f16, bf16   both products by mma.sync m16n8k16: 16 rows do not fill a tile of the 5th-generation tensor cores, whose turn-around through tensor
 //               memory took 2500 cycles for 128 rows here (tensor memory, softmax of one warp, tensor memory again) against 1300 that the memory needs;
 //   f32         FMA: a lane has a cached row and four queries for the scores, four features of the values and all queries for the sum; bound by the chain of a
-//               slice in a warp (1600 instructions, two warps a scheduler, 45 % of the issue slots).
-// 64 sequences of 100 to 8000 rows, 32 heads over 8, 128 features: bf16 184 us of 164 that the memory needs (5.8 TB/s); f32 486 us (4.4 TB/s).
+//               slice in a warp (1600 instructions with eight queries, two warps a scheduler, 45 % of the issue slots).
+// 64 sequences of 100 to 8000 rows, 32 heads over 8, 128 features: bf16 184 us of 164 that the memory needs (5.8 TB/s); f32 403 us (5.3 TB/s).
 // One token of one sequence of 1000 rows, 32 heads of 96 features: 15.3 us, of which the attention 11: items, then a chain of three slices, then the joins.
 // Weights are rounded to the operands' type for the second product, as in paged_attention_tc.cu; values that are masked and not finite are kept out
 // the same way.  Every wait is bounded; a warp whose wait gave up goes through the motions, so that the CTA's barriers are met.
@@ -166,7 +166,9 @@ template <class T> struct Part {
     }
 };
 
-// f32: for the scores lane has cached row lane % 16 of the slice and queries 4 (lane / 16) .. + 3, for the sum features 4 lane .. + 3 of all queries
+// f32: for the scores lane has cached row lane % 16 of the slice and queries 4 (lane / 16) .. + 3, for the sum features 4 lane .. + 3 of all queries.
+// With FEW, up to four queries: a cached row's two lanes have half of its features each, and the same four queries: 64 sequences of 32 heads over 8,
+// 128 features 488 -> 403 us, 64 features 351 -> 309; items of eight rows pay 2.8 % for the longer kernel (64 heads over 8: 486 -> 500).
 template <> struct Part<float> {
     float4 o[8];
     float m[4], l[4];
@@ -181,17 +183,19 @@ template <> struct Part<float> {
         }
     }
     // pos: rows of the lane's queries' tokens (-1: none); qs: the item's queries [8][128]; own: [16][8] weights and [8] factors of the warp's own
+    template <bool FEW>
     __device__ __forceinline__ void step(const RowsArgs& x, const unsigned char* ks, const unsigned char* vs, bool masked, int j, const int (&pos)[4], float* const (&to)[4],
                                          const float* qs, float* own) {
         const AttendArgs& a = x.a;
         const int lane = threadIdx.x & 31, key = lane & 15, rg = lane >> 4;
         float z[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 16
-        for (int c = 0; c < a.p.D / 4; ++c) {
+        for (int i = 0; i < a.p.D / (FEW ? 8 : 4); ++i) {
+            const int c = FEW ? 2 * i + rg : i;
             const float4 k = *reinterpret_cast<const float4*>(ks + piece(key, c));
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float4 q = *reinterpret_cast<const float4*>(qs + (4 * rg + r) * 128 + 4 * c);
+                const float4 q = *reinterpret_cast<const float4*>(qs + (FEW ? r : 4 * rg + r) * 128 + 4 * c);
                 z[r] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, z[r]))));
             }
         }
@@ -199,6 +203,7 @@ template <> struct Part<float> {
         float corr[4], u[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+            if (FEW) z[r] += __shfl_xor_sync(0xffffffffu, z[r], 16);
             z[r] *= a.c;
             const int at = j + key;
             if (masked && (at > pos[r] || (a.window > 0 && at <= pos[r] - a.window && at >= a.first))) z[r] = -INFINITY;
@@ -221,7 +226,7 @@ template <> struct Part<float> {
             const float4 c0 = *reinterpret_cast<const float4*>(own + 128), c1 = *reinterpret_cast<const float4*>(own + 132);
             const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-            for (int r = 0; r < 8; ++r) o[r] = make_float4(o[r].x * c[r], o[r].y * c[r], o[r].z * c[r], o[r].w * c[r]);
+            for (int r = 0; r < (FEW ? 4 : 8); ++r) o[r] = make_float4(o[r].x * c[r], o[r].y * c[r], o[r].z * c[r], o[r].w * c[r]);
         }
         if (4 * lane < a.p.E) {
 #pragma unroll
@@ -230,7 +235,7 @@ template <> struct Part<float> {
                 const float4 p0 = *reinterpret_cast<const float4*>(own + k * 8), p1 = *reinterpret_cast<const float4*>(own + k * 8 + 4);
                 const float w[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
 #pragma unroll
-                for (int r = 0; r < 8; ++r) o[r] = make_float4(fmaf(w[r], v.x, o[r].x), fmaf(w[r], v.y, o[r].y), fmaf(w[r], v.z, o[r].z), fmaf(w[r], v.w, o[r].w));
+                for (int r = 0; r < (FEW ? 4 : 8); ++r) o[r] = make_float4(fmaf(w[r], v.x, o[r].x), fmaf(w[r], v.y, o[r].y), fmaf(w[r], v.z, o[r].z), fmaf(w[r], v.w, o[r].w));
             }
         }
         __syncwarp();
@@ -337,9 +342,9 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int u = 4 * (lane >> 4) + r;
+                const int u = (count > 4 ? 4 * (lane >> 4) : 0) + r;
                 pos[r] = u < count ? row_of(u) : -1;
-                if (x.scores && u < count) to[r] = x.scores + query(u) * room;
+                if (x.scores && u < count && (count > 4 || lane < 16)) to[r] = x.scores + query(u) * room;
             }
             part.begin();
             __syncthreads();
@@ -378,8 +383,10 @@ rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
-            if constexpr (f32) part.step(x, ks, vs, masked, j, pos, to, qs, own[warp]);
-            else part.step(x, smem_u32(ks), smem_u32(vs), masked, j, pos[0], pos[1], to[0], to[1]);
+            if constexpr (f32) {
+                if (count > 4) part.template step<false>(x, ks, vs, masked, j, pos, to, qs, own[warp]);
+                else part.template step<true>(x, ks, vs, masked, j, pos, to, qs, own[warp]);
+            } else part.step(x, smem_u32(ks), smem_u32(vs), masked, j, pos[0], pos[1], to[0], to[1]);
             __syncwarp();
         }
         // the warps' maxima and sums

@@ -61,7 +61,7 @@ using namespace paged;
 
 // ------------------------------------------------------------------------------------------------ append
 // A CTA per token: its sequence, then its row's units of keys and of values.  Reads and writes 2 G (D + E) elements per token, bound by
-// memory for prompts and by the launch for single tokens.
+// memory for prompts (8 heads of 128, bf16, seven prompts of up to 1700 tokens: 14.2 us, 5.0 TB/s) and by the launch for single tokens (96 of them 3.9 us).
 template <class Unit>
 __global__ void __launch_bounds__(128) append_kernel(const View p, const Unit* __restrict__ k, long long k_pitch, const Unit* __restrict__ v, long long v_pitch,
                                                      int du, int eu, int* lengths_out) {
@@ -125,7 +125,8 @@ void launch_append(rcu_device* dev, const View& p, const void* k, uint64_t k_pit
 //   3. In place: rows in order of their new places, as many per round as the cluster's registers hold: read, wait for the cluster, write.  A row's new
 //      place is never behind its old one, so what a round writes has been read in it or before.  Into other arrays: a kernel behind this one, in
 //      which nobody waits (in rounds the copy of 4096 rows of 16 sequences by 8 heads took 130 us, 4.1 TB/s).
-// Bound by memory: the masses (several times, from L2), then 2 keep (D + E) elements.
+// Bound by memory: the masses, then 2 keep (D + E) elements.  4096 of up to 16000 rows, 16 sequences, 8 heads, bf16, 128 features: 132 us, of which the selection 40 (four
+// passes with a barrier of the cluster each), the copy 92 at 6.0 TB/s; 1000 of 2048 rows of one sequence 17.8 us.
 constexpr int kEvictThreads = 256, kEvictUnits = 8, kEvictCluster = 8, kEvictCodes = 6144;
 
 struct EvictArgs {
@@ -423,6 +424,8 @@ rcu_status rcu_paged_evict(rcu_device* dev, const rcu_paged* cache, const rcu_pa
     st = list.take("paged_evict", scratch, rcu_paged_evict_scratch(dev, cache, keep));
     if (st != RCU_OK) return st;
     a.list = (unsigned*)list.ptr;
+    // clusters as large as four CTAs an SM allow, which is what fits: 16 sequences of up to 16000 rows by 8 heads 132 us (two 153, eight 140), of up to 5000 rows
+    // 38.6 (41.9, 49.8); few sequences have clusters of eight in any case
     constexpr long long kPerSm = 4;
     const int pairs = p.S * p.G;
     int cluster = kEvictCluster;
