@@ -642,7 +642,7 @@ template <class T> rcu_status launch(rcu_device* dev, const AttendArgs& a, int d
     plan_of(dev, p, a.H, (char*)scratch, &x.pl);
     x.stage_bytes = (x.nb > x.eb ? x.nb : x.eb) * kBlock;
     constexpr int kTurn = 8 * 2048;
-    const int room = dev->smem_optin - 3072 - kTurn - 2 * x.nb * kBlock;          // 1 KB to align, 2 KB of static shared memory
+    const int room = dev->smem_optin - 3 * 1024 - kTurn - 2 * x.nb * kBlock;          // 1 KB to align, 2 KB of static shared memory
     x.stages = room / x.stage_bytes < kMostStages ? room / x.stage_bytes : kMostStages;
     const size_t smem = 1024 + (size_t)2 * x.nb * kBlock + (size_t)x.stages * x.stage_bytes + kTurn;
     CUtensorMap qm, km, vm;
