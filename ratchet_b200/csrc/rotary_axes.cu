@@ -34,11 +34,16 @@ __device__ __forceinline__ float2 turn_of(const AxesArgs& a, long long t, int i)
 
 // V elements of 16 bytes (VEC), or one by one; TOK tokens per CTA
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) rotary_axes_kernel(const AxesArgs a, const T* x, T* out, int tokens) {
+__global__ void __launch_bounds__(256) rotary_axes_kernel(const AxesArgs a, const T* x, T* out, int tokens, int ahead) {
     rcu_kernel_entry();
     extern __shared__ float2 cs[];
     const long long t0 = (long long)blockIdx.x * tokens;
     const int n = (int)min((long long)tokens, a.T - t0);
+    if (VEC && ahead) {                      // the rows are on their way while the angles are worked out
+        const int lines = (int)(((long long)a.H * a.D * (int)sizeof(T) + 127) / 128);
+        for (int i = threadIdx.x; i < n * lines; i += 256)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(x + (t0 + i / lines) * a.pitch + (long long)(i % lines) * (128 / (int)sizeof(T))));
+    }
     for (int i = threadIdx.x; i < n * a.pairs; i += 256) cs[i] = turn_of(a, t0 + i / a.pairs, i % a.pairs);
     __syncthreads();
     const int lo = a.first, hi = a.first + 2 * a.pairs;
@@ -128,8 +133,11 @@ template <class T> void launch_axes(rcu_device* dev, const AxesArgs& a, const vo
     while (tokens < 8 && (long long)tokens * a.H * a.D < 8 * 256 * V && a.T / (2 * tokens) >= 2 * dev->sm_count && 2 * tokens * a.pairs <= 2048) tokens *= 2;
     const unsigned grid = (unsigned)((a.T + tokens - 1) / tokens);
     const size_t smem = (size_t)tokens * a.pairs * sizeof(float2);
-    if (vec) rcu_launch(dev, rotary_axes_kernel<T, true>, grid, 256, smem, a, (const T*)x, (T*)out, tokens);
-    else rcu_launch(dev, rotary_axes_kernel<T, false>, grid, 256, smem, a, (const T*)x, (T*)out, tokens);
+    // Rows are asked for ahead of the angles where x and dst together are larger than L2, so that x comes from memory: 8192 tokens, 32 heads of 128 in f32 50.4 -> 43.4 us;
+    // with half the heads in f16, which stay in L2, the requests cost 16.4 -> 17.2
+    const int ahead = 2 * a.T * a.H * a.D * (long long)sizeof(T) > (126ll << 20);
+    if (vec) rcu_launch(dev, rotary_axes_kernel<T, true>, grid, 256, smem, a, (const T*)x, (T*)out, tokens, ahead);
+    else rcu_launch(dev, rotary_axes_kernel<T, false>, grid, 256, smem, a, (const T*)x, (T*)out, tokens, ahead);
 }
 
 }  // namespace
