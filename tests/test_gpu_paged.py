@@ -76,6 +76,20 @@ def test_rotary_axes_near_positions_are_exact_to_f32(dev):
     assert np.abs(got - want).max() < 6 * 2.0 ** -24 * np.abs(xv).max()
 
 
+@pytest.mark.parametrize("halves", [False, True])
+def test_rotary_axes_of_more_rows_than_stay_on_chip(dev, halves):
+    """Rows of no whole number of 128-byte lines, a last group of tokens that is not full."""
+    g = rng(11)
+    T, H, D, col = 5203, 41, 80, 4
+    f = 10000.0 ** (-np.arange(40) / 40)
+    hi = f.astype(np.float32)
+    at = g.integers(0, 2 ** 17, (2, T)).astype(np.int32)
+    x, xv = put(dev, g.standard_normal((T, col + H * D)), F32)
+    got = get(dev.rotary_axes(x, H, D, up(dev, np.stack([hi, (f - hi).astype(np.float32)])), up(dev, at), (24, 16), col=col, halves=halves))
+    want = pp.rotary(xv[:, col:].reshape(T, H, D), f, at, (24, 16), 1.0, 0, halves)
+    assert np.abs(got - want).max() < 6 * 2.0 ** -24 * np.abs(xv).max()
+
+
 # ---------------------------------------------------------------------------------------- append
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("new,lengths,G,D,E,R,k_col,v_col", [
