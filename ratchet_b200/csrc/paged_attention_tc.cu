@@ -30,6 +30,11 @@ namespace paged {
 namespace {
 
 constexpr int kThreadsP = 384, kMostStages = 8;
+// A group's notes that a segment has values which are not finite, by the segment's number.  A warp that has passed segment i's meeting may note something
+// of segment i + 1 before a slower one has read what was noted of i, hence not one.  Note i is cleared behind the meeting of i + 1, to which every
+// warp of the group comes with i read; it is next written in segment i + kNotes, and with two notes a warp of that segment could write before a slower
+// one, just past the meeting of i + 1, clears.  With three the meeting of i + 2 lies between.
+constexpr int kNotes = 3;
 
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ View p, const __grid_constant__ Plan pl, int window, int first, int group) {
     rcu_kernel_entry();
@@ -104,7 +109,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
     __shared__ Segment segments[kSegments];
     __shared__ float2 other[kTileQ];                  // maximum and sum that the second group hands to the first
     __shared__ uint32_t tmem_slot;
-    __shared__ volatile int abort_flag, poison[2];
+    __shared__ volatile int abort_flag, poison[2][kNotes];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -132,7 +137,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
             mbar_init(&pv_done[i], 1);
             mbar_init(&o_full[i], 1);
             mbar_init(&met[i], 4);
-            poison[i] = 0;
+            for (int k = 0; k < kNotes; ++k) poison[i][k] = 0;
         }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -355,6 +360,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         for (int i = 0;; ++i) {
             const Segment& seg = take(i, ok);
             if (!ok || !seg.more) break;
+            const int note = i % kNotes;
             const bool two = seg.two;
             const Item it = seg.it;
             const Sight see = seg.see[w];            // copies: what is in shared memory is read again behind every wait
@@ -386,7 +392,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                         if (behind) *at = make_uint4(0, 0, 0, 0);
                         else bad |= not_finite<T>(u.x) | not_finite<T>(u.y) | not_finite<T>(u.z) | not_finite<T>(u.w);
                     }
-                    if (bad) poison[w] = 1;
+                    if (bad) poison[w][note] = 1;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
 #pragma unroll 1
@@ -471,6 +477,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
             ok = wait(bar, two ? meets++ : joins);
             if (!ok) break;
             tc_fence_after();
+            if (lane == 0) poison[w][note == 0 ? kNotes - 1 : note - 1] = 0;          // what the segment before noted: all have read it (kNotes)
             if (!two && w == 1) {
                 ok = wait(&taken, joins++);
                 if (!ok) break;
@@ -491,19 +498,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
 #pragma unroll 1
                 for (int n = seg.n0 + 1; n < n1 && !both; n += 2) both = seg.see[0](n);
             }
-            if (poison[w] || (!two && poison[1])) {
+            // the second group, which goes on behind `taken` alone, writes no note of its own before this one has been read
+            if (poison[w][note] || (!two && poison[1][note])) {
                 if (live) redo_rows<T>(x, seg, w, quarter);
-#pragma unroll 1
-                for (int k = 0; k < 2 && ok; ++k) {             // all have read the note; all see it taken back
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&met[w]);
-                    ok = wait(&met[w], meets++);
-                    if (k == 0) {
-                        poison[w] = 0;
-                        if (!two) poison[1] = 0;
-                    }
-                }
-                if (!ok) break;
             } else if (live) {
                 const int h = seg.g * x.group + head, part_row = (two ? w : 0) * kTileQ + r;
                 float inv = scale0;

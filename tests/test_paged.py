@@ -90,3 +90,75 @@ def test_builders_refuse_what_does_not_fit():
     assert axes(2, 2, 64, 0, at, sec(10, 5)) == capi.ERR_INVALID_ARG                   # a pair without an axis
     assert axes(2, 2, 64, 0, leaf(F32, 2, 5), sec(10, 6)) == capi.ERR_INVALID_ARG
     assert axes(2, 2, 64, 0, leaf(I32, 2, 4), sec(10, 6)) == capi.ERR_INVALID_ARG
+
+
+# ---------------------------------------------------------------------------------------- notes of values that are not finite
+class Meeting:
+    def __init__(self, count):
+        self.count, self.arrived, self.phase = count, 0, 0
+
+    def arrive(self):
+        self.arrived += 1
+        if self.arrived == self.count:
+            self.arrived, self.phase = 0, self.phase + 1
+
+
+def group_of_warps(seed, notes, segments=40, warps=4):
+    """The softmax warps of one query tile (paged_attention_tc.cu) as far as their notes go, each as far as its waits let it, in an order drawn from `seed`:
+    the number of segments for which a warp read another note than what the tile's warps wrote of that segment, and whether all ended.
+    notes 0: one note, which the warps take back at two further meetings where it is set."""
+    import random
+    r = random.Random(seed)
+    bad = [[r.random() < 0.15 for _ in range(warps)] for _ in range(segments)]
+    idle = [r.random() < 0.5 for _ in range(warps)]                       # warps without a query do nothing between the meetings
+    note, met, wrong = [False] * max(1, notes), Meeting(warps), [0]
+
+    def warp(w):
+        phase = 0
+        for i in range(segments):
+            at = i % notes if notes else 0
+            yield
+            if bad[i][w]:
+                note[at] = True
+            yield
+            met.arrive()
+            phase += 1
+            while met.phase < phase:
+                yield
+            if notes:
+                yield
+                note[(at - 1) % notes] = False
+            yield
+            got = note[at]
+            wrong[0] += got != any(bad[i])
+            if not notes and got:
+                for k in range(2):
+                    met.arrive()
+                    phase += 1
+                    while met.phase < phase:
+                        yield
+                    if k == 0:
+                        note[0] = False
+            for _ in range(0 if idle[w] else r.randrange(12)):            # sums to the output, or row by row
+                yield
+
+    running = [warp(w) for w in range(warps)]
+    for _ in range(40000):
+        if not running:
+            return wrong[0], True
+        g = r.choice(running)
+        if next(g, running) is running:
+            running.remove(g)
+    return wrong[0], False
+
+
+def test_every_warp_reads_what_its_segment_noted():
+    import re
+    from pathlib import Path
+    source = (Path(__file__).resolve().parent.parent / "ratchet_b200" / "csrc" / "paged_attention_tc.cu").read_text()
+    notes = int(re.search(r"constexpr int kNotes = (\d+);", source).group(1))
+    assert re.search(r"poison\[w\]\[note == 0 \? kNotes - 1 : note - 1\] = 0;", source) and "poison[2][kNotes]" in source
+    assert all(group_of_warps(seed, notes) == (0, True) for seed in range(300))
+    # the model finds what fewer notes do: one read for the wrong segment, warps that wait for one another for good
+    assert any(group_of_warps(seed, 2)[0] for seed in range(300))
+    assert any(not group_of_warps(seed, 0)[1] for seed in range(300))
