@@ -293,21 +293,24 @@ __global__ void __launch_bounds__(kThreadsM, 1) mass_tc_kernel(const __grid_cons
                     float z[64];
                     tmem_ld_32x64(tmem + 128 * t + 64 * half + lanes, z);
                     const float4* ls = reinterpret_cast<const float4*>(&lse[s][64 * half]);
-                    if (!whole) {
-                        asm volatile("" ::: "memory");          // a branch, not 64 predicated selections in every tile
-#pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c < from - 64 * half || c >= upto - 64 * half) z[c] = -INFINITY;
-                    }
                     const float2 c2 = make_float2(a.c, a.c);
+                    auto weights = [&](auto masked) {
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        const float4 v = ls[c];
-                        const float2 x0 = fma2(make_float2(z[4 * c], z[4 * c + 1]), c2, make_float2(v.x, v.y)), x1 = fma2(make_float2(z[4 * c + 2], z[4 * c + 3]), c2, make_float2(v.z, v.w));
-                        add[0] = add2(add[0], make_float2(ex2(x0.x), ex2(x0.y)));
-                        // every fourth pair on the FMA pipe, which takes that off the exponential unit
-                        add[1] = add2(add[1], c & 1 ? ex2_fma(x1) : make_float2(ex2(x1.x), ex2(x1.y)));
-                    }
+                        for (int c = 0; c < 16; ++c) {
+                            const float4 v = ls[c];
+                            float2 x[2] = {fma2(make_float2(z[4 * c], z[4 * c + 1]), c2, make_float2(v.x, v.y)), fma2(make_float2(z[4 * c + 2], z[4 * c + 3]), c2, make_float2(v.z, v.w))};
+                            // behind lse: a query that has none (NaN, or minus infinity for all it sees) must not reach the rows that it does not see
+                            auto seen = [&](int i) { return 4 * c + i >= from - 64 * half && 4 * c + i < upto - 64 * half; };
+                            if (masked())
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) x[i] = make_float2(seen(2 * i) ? x[i].x : -INFINITY, seen(2 * i + 1) ? x[i].y : -INFINITY);
+                            add[0] = add2(add[0], make_float2(ex2(x[0].x), ex2(x[0].y)));
+                            // every fourth pair on the FMA pipe, which takes that off the exponential unit
+                            add[1] = add2(add[1], c & 1 ? ex2_fma(x[1]) : make_float2(ex2(x[1].x), ex2(x[1].y)));
+                        }
+                    };
+                    if (whole) weights(std::false_type{});          // a branch, not 64 selections in every tile
+                    else weights(std::true_type{});
                 }
                 tc_fence_before();
                 const float2 both = add2(add[0], add[1]);

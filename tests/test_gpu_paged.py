@@ -213,6 +213,48 @@ def test_many_short_sequences_some_with_values_that_are_not_finite(dev, dt, new,
 
 
 @pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("what", ["query", "key"])
+@pytest.mark.parametrize("n,L,D,window", [(70, 300, 64, 0), (70, 300, 64, 25), (200, 200, 80, 40), (4, 60, 64, 3), (9, 40, 136, 4)])
+def test_a_token_without_a_softmax_has_no_part_in_the_sums_of_rows_that_it_does_not_see(dev, dt, what, n, L, D, window):
+    """A query of NaN, and one that has minus infinity for every row that it sees: the rows that it sees receive NaN, all others what the other tokens give."""
+    g = rng(n + L)
+    H, G = 4, 2
+    at = n // 3
+    c = pp.Cache(g, dt, [n], [L], G, D, D, 16)
+    h, qv = pp.encode(g.standard_normal((n, H, D)), dt)
+    keys = pp.decode(c.keys, dt)
+    odd = np.zeros((n, G), bool)                            # tokens without a softmax in one of the group's heads
+    if what == "query":
+        qv[at, 3] = np.nan
+        odd[at, 1] = True
+    else:
+        qv[:, 2:, 0] = 1.0
+        for r in range(L - n + at + 1):                     # all that the token sees, and those before it
+            c.k[0][r, 1, 0] = keys[c.table[0, r // 16], 1, r % 16, 0] = -np.inf
+        vis = pp.seen(L, n, window, 0)
+        odd[:, 1] = [not vis[i, L - n + at + 1:].any() for i in range(n)]
+    q = up(dev, pp.encode(qv, dt)[0], dt)
+    c.keys = pp.encode(keys, dt)[0]
+    want, vis = np.zeros((G, L)), np.broadcast_to(pp.seen(L, n, window, 0), (n, L))
+    for head in range(H):
+        for i in range(n):
+            rows = np.flatnonzero(vis[i])
+            with np.errstate(invalid="ignore"):
+                z = 0.125 * c.k[0][rows, head // 2] @ qv[i, head]
+                w = np.exp(z - z.max())
+                want[head // 2, rows] += w / w.sum()
+    assert np.isnan(want).any() and np.isfinite(want).any()
+    assert np.array_equal(np.isnan(want), np.stack([(odd[:, k, None] & vis).any(0) for k in range(G)]))
+    d = device_cache(dev, c, np.zeros((1, G, c.rows)))
+    dev.paged_attention(q, d, 0.125, window=window)
+    got = d.mass.to_numpy()[0, :, :L].astype(np.float64)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = np.isfinite(want)
+    assert np.all(np.abs(got - want)[fine] <= 2e-5 * want[fine] + 4 * 2.0 ** -24 * (1 + want[fine]))
+    dev.sync()
+
+
+@pytest.mark.parametrize("dt", DTS)
 def test_attention_leaves_rows_of_no_sequence(dev, dt):
     g = rng(11)
     c = pp.Cache(g, dt, [3, 5], [30, 5], 2, 64, 64, 16)
