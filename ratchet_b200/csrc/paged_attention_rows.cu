@@ -10,8 +10,8 @@
 //               slice in a warp (1600 instructions with eight queries, two warps a scheduler, 45 % of the issue slots).
 // 64 sequences of 100 to 8000 rows, 32 heads over 8, 128 features: bf16 184 us of 164 that the memory needs (5.8 TB/s); f32 403 us (5.3 TB/s).
 // One token of one sequence of 1000 rows, 32 heads of 96 features: 15.3 us, of which the attention 11: items, then a chain of three slices, then the joins.
-// Weights are rounded to the operands' type for the second product, as in paged_attention_tc.cu; values that are masked and not finite are kept out
-// the same way.  Every wait is bounded; a warp whose wait gave up goes through the motions, so that the CTA's barriers are met.
+// Weights are rounded to the operands' type for the second product and taken against the maximum less 7 in f16, as in paged_attention_tc.cu; values that are masked and not
+// finite are kept out the same way.  Every wait is bounded; a warp whose wait gave up goes through the motions, so that the CTA's barriers are met.
 #include "paged_rows.cuh"
 #include "paged_tc.cuh"
 
@@ -116,7 +116,7 @@ template <class T> struct Part {
         for (int h = 0; h < 2; ++h) {
             float top = fmaxf(fmaxf(z[0][2 * h], z[0][2 * h + 1]), fmaxf(z[1][2 * h], z[1][2 * h + 1]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) - Above<T>::value;
             // the maximum only moves when a score exceeds it by more than 2^8
             const bool move = top > m[h] + 8.f || (m[h] == -INFINITY && top > -INFINITY);
             corr[h] = move ? ex2(m[h] - top) : 1.f;

@@ -11,8 +11,8 @@
 //                       while the weights of the other are worked out.  The maximum that weights are taken against only moves when a score exceeds
 //                       it by more than 2^8, so that O_w is rescaled rarely.
 // An item of one query tile (generation) gives it to both groups, which take the tiles of rows in turns and join their sums at the end.
-// Weights enter the second product in the operands' type: half a step of theirs moves the sum by as much as the rounding of the output does.  Their
-// sum, the maximum and O are f32.
+// Weights enter the second product in the operands' type, which the matrix instructions want: each is off by half a step of itself at most, the output by half a
+// step of sum p |v| (paged_tc.cuh has how f16 weights keep out of the type's small numbers).  Their sum, the maximum and O are f32.
 // What is masked must not reach the sum even where it is not finite, and 0 times infinity is NaN.  Rows behind the sequence's last one are zeroed in
 // shared memory.  In a tile that some of the queries see in part, an infinity or NaN among the values sends the query tile to attend_rows, which
 // reads only what each query sees.
@@ -416,7 +416,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                         for (int j = 4; j < 60; j += 8)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], s[j + e], s[j + 4 + e]);
-                        const float top = max3(max3(top4[0], top4[1], top4[2]), max3(top4[3], s[60], s[61]), fmaxf(s[62], s[63])) * a.c;      // c > 0
+                        const float top = max3(max3(top4[0], top4[1], top4[2]), max3(top4[3], s[60], s[61]), fmaxf(s[62], s[63])) * a.c - Above<T>::value;      // c > 0
                         const bool move = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
                         const float next = move ? top : m;
                         const float corr = move ? ex2(m - next) : 1.f;                    // 0 while no key has been seen

@@ -25,6 +25,12 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
     const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Weights are taken against the running maximum less this (units of log 2), which stands for the maximum from there on: in the sums, the parts and lse.  f16's smallest
+// step is 2^-24, and a weight below half of it vanishes: one row 17 above 20000 others would be all there is (an output of 0.05 was off by 2.8e-4, eleven half steps).
+// Against the maximum less 7, weights lie below 2^15 (the maximum moves by steps of more than 8) and are off by 2^-32 of the largest at most; 131000 of them by
+// 2^-15 of the sum together.  bf16 has f32's range.
+template <class T> struct Above { static constexpr float value = 0.f; };
+template <> struct Above<__half> { static constexpr float value = 7.f; };
 // whether one of the two 16-bit values is an infinity or NaN
 template <class T> __device__ __forceinline__ uint32_t not_finite(uint32_t x);
 template <> __device__ __forceinline__ uint32_t not_finite<__half>(uint32_t x) { return __vcmpgeu2(x & 0x7fff7fffu, 0x7c007c00u); }

@@ -254,6 +254,30 @@ def test_a_token_without_a_softmax_has_no_part_in_the_sums_of_rows_that_it_does_
     dev.sync()
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("n,L", [(1, 131000), (8, 20008), (64, 20064)])
+def test_attention_under_a_row_far_above_all_others(dev, dt, n, L):
+    """A first row 17 above all others, as language models have it: the weights of the others are 2^-25 of its own, and together they are what an f16's half step
+    of the output would show.  Every sequence reads the same pages, so that each CTA has whole items: a few rows each, one query tile, and two."""
+    g = rng(n)
+    S, H, G, D, R = 40, 16, 4, 16, 256
+    c = pp.Cache(g, dt, [n], [16], G, D, D, R, spare=0)          # its rows are made below: as many as that one by one take a while
+    pages = -(-L // R)
+    k, v = 0.1 * g.standard_normal((pages * R, G, D)), 0.25 + 0.75 * g.random((pages * R, G, D))
+    k[0], v[0] = 4.35, 0.05
+    hk, k = pp.encode(k, dt)
+    hv, v = pp.encode(v, dt)
+    paged = lambda a: np.ascontiguousarray(a.reshape(pages, R, G, D).transpose(0, 2, 1, 3))  # noqa: E731
+    c.keys, c.values, c.k, c.v, c.lengths = paged(hk), paged(hv), [k[:L]], [v[:L]], [L]
+    hq, qv = pp.encode(1 + 0.01 * g.standard_normal((n, H, D)), dt)
+    want, size, _ = pp.attention(c, qv, 0.25)
+    assert 0.9 < np.exp(-17.4) * (L - n) * 0.625 / (want.mean() - 0.05) < 1.3 or dt == BF16
+    c.table, c.lengths = np.tile(np.arange(pages, dtype=np.int32), (S, 1)), [L] * S
+    c.starts = (n * np.arange(S + 1)).astype(np.int32)
+    got = get(dev.paged_attention(up(dev, np.tile(hq, (S, 1, 1)), dt), device_cache(dev, c), 0.25)).reshape(S, n, H, D)
+    assert all(close(got[s], want, size, dt, 1.0) for s in range(S))
+
+
 @pytest.mark.parametrize("dt", DTS)
 def test_attention_leaves_rows_of_no_sequence(dev, dt):
     g = rng(11)
