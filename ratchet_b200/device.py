@@ -81,8 +81,26 @@ class PagedCache:
 
     def __init__(self, keys: Buffer, values: Buffer, table: Buffer, lengths: Buffer, starts: Optional[Buffer] = None, mass: Optional[Buffer] = None):
         self.keys, self.values, self.table, self.starts, self.lengths, self.mass = keys, values, table, starts, lengths, mass
-        self.struct = capi.rcu_paged(*(b.desc() if b is not None else capi.rcu_tensor() for b in (keys, values, table, starts, lengths, mass)))
-        self.ref = C.byref(self.struct)
+        self._named = self._owners = self._ref = None
+
+    @property
+    def ref(self):
+        """The descriptor for the C ABI, of the buffers as they are now: one that was put in another's place counts, and one that was freed is refused (a
+        structure made earlier would still name its block, which the pool may have handed on)."""
+        named = (self.keys, self.values, self.table, self.starts, self.lengths, self.mass)
+        if named != self._named or not all([b.ptr for b in self._owners]):
+            owners = [b._base or b for b in named if b is not None]
+            for b in owners:
+                if not b.ptr:
+                    self._named = None
+                    raise RatchetCudaError(capi.ERR_INVALID_ARG, "paged cache: a buffer of it has been freed")
+            self._ref = C.byref(capi.rcu_paged(*(capi.rcu_tensor() if b is None else b.desc() for b in named)))
+            self._named, self._owners = named, owners
+        return self._ref
+
+    @property
+    def struct(self) -> capi.rcu_paged:
+        return self.ref._obj
 
 
 class Device:

@@ -92,6 +92,54 @@ def test_builders_refuse_what_does_not_fit():
     assert axes(2, 2, 64, 0, leaf(I32, 2, 4), sec(10, 6)) == capi.ERR_INVALID_ARG
 
 
+# ---------------------------------------------------------------------------------------- handles
+class Pool:
+    """A device's part in a buffer's life."""
+
+    def __init__(self):
+        self.freed = []
+
+    def _free(self, ptr):
+        self.freed.append(ptr)
+
+
+@pytest.mark.parametrize("name", ["keys", "values", "table", "lengths", "starts", "mass"])
+@pytest.mark.parametrize("view", [False, True])
+def test_a_cache_names_its_buffers_as_they_are(name, view):
+    from ratchet_b200 import Buffer, PagedCache, RatchetCudaError, capi
+    dev = Pool()
+    shapes = {"keys": (4, 2, 16, 64), "values": (4, 2, 16, 64), "table": (2, 2), "lengths": (2,), "starts": (3,), "mass": (2, 2, 32)}
+    types = {"keys": capi.F16, "values": capi.F16, "mass": capi.F32}
+    made = {n: Buffer(dev, types.get(n, capi.I32), s, 0x1000 * (i + 1), 64, True) for i, (n, s) in enumerate(shapes.items())}
+    c = PagedCache(**{n: b.view(b.shape) if view else b for n, b in made.items()})
+    assert [getattr(c.struct, n).data for n in shapes] == [b.ptr for b in made.values()]
+    assert c.ref is c.ref                                   # made once while nothing changes
+    other = Buffer(dev, made[name].dt, made[name].shape, 0x9000, 64, True)
+    kept = getattr(c, name)
+    setattr(c, name, other)
+    assert getattr(c.struct, name).data == 0x9000
+    setattr(c, name, kept)
+    assert getattr(c.struct, name).data == made[name].ptr
+    c.ref
+    made[name].free()
+    for _ in range(2):
+        with pytest.raises(RatchetCudaError):
+            c.ref
+    with pytest.raises(RatchetCudaError):
+        c.struct
+    setattr(c, name, other)
+    assert getattr(c.struct, name).data == 0x9000
+    with pytest.raises(RatchetCudaError):
+        PagedCache(**{n: made.get(n) for n in shapes}).ref
+
+
+def test_a_cache_without_starts_and_sums():
+    from ratchet_b200 import Buffer, PagedCache, capi
+    b = lambda dt, *s: Buffer(None, dt, s, 0x1000, 64, False)  # noqa: E731
+    c = PagedCache(b(capi.F16, 4, 2, 16, 64), b(capi.F16, 4, 2, 16, 64), b(capi.I32, 2, 2), b(capi.I32, 2))
+    assert c.struct.starts.data is None and c.struct.mass.data is None and c.struct.keys.shape[1] == 2
+
+
 # ---------------------------------------------------------------------------------------- notes of values that are not finite
 class Meeting:
     def __init__(self, count):
