@@ -409,7 +409,9 @@ rcu_status rcu_lazy_window_attention(rcu_lazy* q, rcu_lazy* kv, rcu_lazy* shared
 
 /* Paged caches as nodes.  keys, values, table, starts, mass (nullable) are resolved tensors; what a node writes to them is a side effect.
  * rcu_lazy_paged_append and rcu_lazy_paged_evict give the sequences' lengths as they are behind the node, I32 [sequences]: who reads the
- * cache after them takes that tensor as its `lengths`. */
+ * cache after them takes that tensor as its `lengths`.  Nodes over the same pages or sums run in the order in which they were built, whichever is
+ * resolved first: where one writes what another reads or writes, the later one has the earlier as a further source (and holds it) as long as that
+ * has not been resolved.  A node that was released unresolved does not run. */
 rcu_status rcu_lazy_rotary_axes(rcu_lazy* x, uint32_t x_col, uint32_t heads, uint32_t dim, uint32_t first, rcu_lazy* freqs, float magnitude,
                                 rcu_lazy* positions, const uint32_t* sections, int halves, rcu_lazy** out);
 rcu_status rcu_lazy_paged_append(rcu_lazy* k, uint32_t k_col, rcu_lazy* v, uint32_t v_col, rcu_lazy* keys, rcu_lazy* values, rcu_lazy* table,

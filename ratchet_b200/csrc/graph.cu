@@ -22,6 +22,7 @@
 #include <atomic>
 #include <deque>
 #include <memory>
+#include <mutex>
 
 #include <cstdio>
 
@@ -66,6 +67,7 @@ struct rcu_lazy {
     uint32_t rank = 1;
     uint64_t shape[RCU_MAX_RANK] = {1, 1, 1, 1};
     std::vector<rcu_lazy*> srcs;   // each entry holds one reference
+    size_t own = 0;                // of a node over a paged cache: the sources that it takes; those behind them only come before it (order_paged)
     // op parameters
     int op = 0;                    // binary / unary op, norm kind
     int flags[3] = {0, 0, 0};      // matmul transposes
@@ -96,6 +98,77 @@ namespace {
 
 void retain(rcu_lazy* t) { t->refs.fetch_add(1, std::memory_order_relaxed); }
 
+// Nodes over paged caches that may have no result yet, in the order in which they were built; no references are held.  Their effects are on pages and sums, not in
+// what they return, so the graph's edges alone do not say which comes first: an eviction takes the lengths that an append gives, and would run ahead of the
+// attention whose weights it goes by.
+struct PagedNodes {
+    std::mutex mutex;
+    std::vector<rcu_lazy*> nodes;
+};
+PagedNodes& paged_nodes() {
+    static PagedNodes* p = new PagedNodes();          // outlives whatever is released at exit
+    return *p;
+}
+bool is_paged(int kind) { return kind == K_PAGED_APPEND || kind == K_PAGED_ATTENTION || kind == K_PAGED_EVICT; }
+
+// The sources whose memory a node over a paged cache reads, as pages and sums, and writes
+struct Touched {
+    int reads[3], writes[3], nr = 0, nw = 0;
+    explicit Touched(const rcu_lazy* t) {
+        auto r = [&](int i) { reads[nr++] = i; };
+        auto w = [&](int i) { writes[nw++] = i; };
+        switch (t->kind) {
+            case K_PAGED_APPEND: w(2); w(3); if (t->flags[0]) w(7); break;
+            case K_PAGED_ATTENTION: r(1); r(2); if (t->flags[0]) w(6); break;
+            case K_PAGED_EVICT: r(0); r(1); r(4); w(5); w(6); w(8); break;
+            default: break;
+        }
+    }
+};
+
+// Whether `late` has to come after `early`
+bool follows(const rcu_lazy* early, const rcu_lazy* late) {
+    const Touched a(early), b(late);
+    auto meet = [&](int x, int y) {
+        const rcu_lazy *s = early->srcs[x], *t = late->srcs[y];
+        const char *p = (const char*)s->storage->ptr, *q = (const char*)t->storage->ptr;
+        return p < q + t->nbytes() && q < p + s->nbytes();
+    };
+    for (int i = 0; i < a.nw; ++i) {
+        for (int j = 0; j < b.nr; ++j)
+            if (meet(a.writes[i], b.reads[j])) return true;
+        for (int j = 0; j < b.nw; ++j)
+            if (meet(a.writes[i], b.writes[j])) return true;
+    }
+    for (int i = 0; i < a.nr; ++i)
+        for (int j = 0; j < b.nw; ++j)
+            if (meet(a.reads[i], b.writes[j])) return true;
+    return false;
+}
+
+// A node over a paged cache comes after the ones that were built before it and have no result yet, where one of the two writes what the other reads or writes: these
+// become further sources, behind the ones that it takes.
+void order_paged(rcu_lazy* n) {
+    PagedNodes& all = paged_nodes();
+    n->own = n->srcs.size();
+    const std::lock_guard<std::mutex> lock(all.mutex);
+    all.nodes.erase(std::remove_if(all.nodes.begin(), all.nodes.end(), [](const rcu_lazy* t) { return t->resolved(); }), all.nodes.end());
+    for (rcu_lazy* t : all.nodes) {
+        if (t->dev != n->dev || std::find(n->srcs.begin(), n->srcs.end(), t) != n->srcs.end() || !follows(t, n)) continue;
+        uint32_t refs = t->refs.load(std::memory_order_relaxed);
+        while (refs && !t->refs.compare_exchange_weak(refs, refs + 1, std::memory_order_relaxed)) {}
+        if (refs) n->srcs.push_back(t);               // one that is being released right now waits for the lock
+    }
+    all.nodes.push_back(n);
+}
+
+void forget_paged(rcu_lazy* n) {
+    PagedNodes& all = paged_nodes();
+    const std::lock_guard<std::mutex> lock(all.mutex);
+    const auto at = std::find(all.nodes.rbegin(), all.nodes.rend(), n);
+    if (at != all.nodes.rend()) all.nodes.erase(std::next(at).base());
+}
+
 void release(rcu_lazy* t) {
     // iterative: a long chain of nodes must not recurse through destructors
     std::vector<rcu_lazy*> work{t};
@@ -103,6 +176,7 @@ void release(rcu_lazy* t) {
         rcu_lazy* n = work.back();
         work.pop_back();
         if (n->refs.fetch_sub(1, std::memory_order_acq_rel) == 1) {
+            if (is_paged(n->kind)) forget_paged(n);
             for (rcu_lazy* s : n->srcs) work.push_back(s);
             delete n;
         }
@@ -390,7 +464,7 @@ rcu_status run_node(rcu_lazy* n, void* converted) {
         }
         case K_PAGED_APPEND: {      // k, v, keys, values, table, starts, lengths, [mass]
             rcu_tensor k = S(0), v = S(1);
-            const rcu_paged c{S(2), S(3), S(4), S(5), S(6), n->srcs.size() > 7 ? S(7) : rcu_tensor{}};
+            const rcu_paged c{S(2), S(3), S(4), S(5), S(6), n->flags[0] ? S(7) : rcu_tensor{}};
             return rcu_paged_append_to(dev, &k, n->u[0], &v, n->u[1], &c, (int*)dst.data);
         }
         case K_PAGED_ATTENTION: {   // q, keys, values, table, starts, lengths, [mass], [sink]
@@ -837,6 +911,14 @@ rcu_status resolve(rcu_lazy* out) {
     if (log)
         std::fprintf(stderr, "[rcu] resolve: %zu nodes, %u launches, %u in place, %zu buffers, %llu bytes planned (%llu unshared), %u weights converted beside a product\n", n,
                      dev->last_resolve.launched, n_inplace, objects.size(), (unsigned long long)planned, (unsigned long long)naive, beside.started);
+    // who only came before has come: a cache that is always a step ahead of its resolves would hold every step's outputs
+    std::vector<rcu_lazy*> before;
+    for (rcu_lazy* t : order)
+        if (is_paged(t->kind) && t->srcs.size() > t->own) {
+            before.insert(before.end(), t->srcs.begin() + t->own, t->srcs.end());
+            t->srcs.resize(t->own);
+        }
+    for (rcu_lazy* t : before) release(t);
     return RCU_OK;
 }
 
@@ -1337,6 +1419,8 @@ rcu_status rcu_lazy_paged_append(rcu_lazy* k, uint32_t k_col, rcu_lazy* v, uint3
     rcu_lazy* n = new_node(dev, K_PAGED_APPEND, RCU_I32, 1, lengths->shape, {k, v, keys, values, table, starts, lengths, mass});
     n->u[0] = k_col;
     n->u[1] = v_col;
+    n->flags[0] = mass != nullptr;
+    order_paged(n);
     *out = n;
     return RCU_OK;
 }
@@ -1355,6 +1439,7 @@ rcu_status rcu_lazy_paged_attention(rcu_lazy* q, rcu_lazy* keys, rcu_lazy* value
     n->u[0] = window;
     n->u[1] = first;
     n->f[0] = scale;
+    order_paged(n);
     *out = n;
     return RCU_OK;
 }
@@ -1371,6 +1456,7 @@ rcu_status rcu_lazy_paged_evict(rcu_lazy* keys, rcu_lazy* values, rcu_lazy* tabl
     n->u[0] = keep;
     n->u[1] = first;
     n->u[2] = recent;
+    order_paged(n);
     *out = n;
     return RCU_OK;
 }

@@ -569,9 +569,11 @@ struct Pass {
                 case K_CACHE: case K_INDEX_WRITE: writes(0); break;
                 case K_LIGHTNING: writes(2); break;
                 case K_LATENT_APPEND: case K_KV_APPEND: writes(3); break;
-                case K_PAGED_APPEND: writes(2); writes(3); if (t->srcs.size() > 7) writes(7); break;
-                case K_PAGED_ATTENTION: if (t->flags[0]) writes(6); break;
-                case K_PAGED_EVICT: writes(5); writes(6); writes(8); break;
+                case K_PAGED_APPEND: case K_PAGED_ATTENTION: case K_PAGED_EVICT: {
+                    const Touched touched(t);
+                    for (int k = 0; k < touched.nw; ++k) writes(touched.writes[k]);
+                    break;
+                }
                 default: break;
             }
         }

@@ -176,7 +176,7 @@ class SequenceState:
 class PagedState:
     """Graph tensors of a paged cache: pages of keys and values [pages, kv_heads, page_rows, features], the table I32 [sequences, max_pages], starts
     I32 [sequences + 1] of a step's new tokens, lengths I32 [sequences] with them, and (optional) the attention weight F32 [sequences,
-    kv_heads, max_pages * page_rows] that every row has received."""
+    kv_heads, max_pages * page_rows] that every row has received.  Nodes over the same pages run in the order in which they were built."""
 
     def __init__(self, keys, values, table, starts, lengths, mass=None):
         self.keys, self.values, self.table, self.starts, self.lengths, self.mass = keys, values, table, starts, lengths, mass

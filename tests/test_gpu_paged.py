@@ -489,6 +489,76 @@ def test_a_run_of_the_graph(dev, dt):
     serve(dev, dt, step, evict)
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("steps", [1, 3])
+def test_a_graph_whose_eviction_is_resolved_first(dev, dt, steps):
+    """Append, attention with sums and eviction in place, of one step or three, all unresolved, each step's lengths from the host: the last eviction is resolved first and
+    the outputs from the last to the first; outputs and weights are those of the order in which the nodes were built."""
+    g = rng(19)
+    H, G, D, R, MP, keep, first, recent = 4, 2, 64, 16, 8, 30, 2, 9
+    leaf = lambda a, t=None: Tensor.from_data(a, device=dev, dt=t)  # noqa: E731
+    table = leaf(g.permutation(3 * MP).reshape(3, MP).astype(np.int32))
+    pages = pp.encode(np.zeros((3 * MP, G, R, D)), dt)[0]
+    keys, values, mass = leaf(pages, dt), leaf(pages, dt), leaf(np.zeros((3, G, MP * R), np.float32))
+    k64, v64, m64 = [np.zeros((0, G, D))] * 3, [np.zeros((0, G, D))] * 3, [np.zeros((G, 0))] * 3
+    outs, wants = [], []
+    for new in [[50, 20, 41], [9, 1, 30], [1, 33, 1]][:steps]:
+        T = sum(new)
+        q, k, v = (pp.encode(g.standard_normal((T, n * D)), dt) for n in (H, G, G))
+        c = pp.Cache.__new__(pp.Cache)
+        c.dt, c.new, c.G, c.D, c.E, c.R = dt, new, G, D, D, R
+        c.starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        for s, n in enumerate(new):
+            rows = slice(c.starts[s], c.starts[s] + n)
+            k64[s], v64[s] = np.concatenate([k64[s], k[1][rows].reshape(n, G, D)]), np.concatenate([v64[s], v[1][rows].reshape(n, G, D)])
+            m64[s] = np.concatenate([m64[s], np.zeros((G, n))], 1)
+        c.k, c.v, c.lengths = list(k64), list(v64), [len(x) for x in k64]
+        want, size, grown = pp.attention(c, q[1].reshape(T, H, D), 0.125)
+        wants.append((want, size))
+        for s, L in enumerate(c.lengths):
+            m = m64[s] + grown[s]
+            at = [pp.kept(m[h], L, keep, first, recent) for h in range(G)]
+            k64[s], v64[s] = (np.stack([x[s][at[h], h] for h in range(G)], 1) for x in (k64, v64))
+            m64[s] = np.stack([m[h, at[h]] for h in range(G)])
+        state = nn.PagedState(keys, values, table, leaf(c.starts), leaf(np.asarray(c.lengths, np.int32)), mass)
+        after = leaf(k[0], dt).paged_append(leaf(v[0], dt), state)
+        outs.append(leaf(q[0].reshape(T, H, D), dt).paged_attention(after, 0.125))
+        cut = after.evict(nn.PagedState(keys, values, table, None, None, mass), keep, first, recent).lengths
+        lengths = np.minimum(c.lengths, keep)
+        del state, after
+    assert np.array_equal(cut.to_numpy(), lengths)
+    sums, got_k, got_v = mass.to_numpy(), pp.decode(keys.to_numpy(), dt), pp.decode(values.to_numpy(), dt)
+    ids = table.to_numpy()
+    for s, L in enumerate(lengths):
+        assert np.allclose(sums[s, :, :L], m64[s], rtol=1e-4, atol=1e-6)
+        for r in range(L):
+            assert np.array_equal(got_k[ids[s, r // R], :, r % R], k64[s][r]) and np.array_equal(got_v[ids[s, r // R], :, r % R], v64[s][r])
+    for o, (want, size) in reversed(list(zip(outs, wants))):
+        assert close(pp.decode(o.to_numpy(), dt).reshape(want.shape), want, size, dt, 5.0)
+    dev.sync()
+
+
+def test_a_graph_that_is_a_step_ahead_keeps_no_outputs(dev):
+    """Every step is built before the one ahead of it is resolved: nodes that only come before let go of one another once they have run."""
+    g = rng(29)
+    leaf = lambda a: Tensor.from_data(a, device=dev)  # noqa: E731
+    keys, values, mass = leaf(np.zeros((40, 2, 16, 64), np.float16)), leaf(np.zeros((40, 2, 16, 64), np.float16)), leaf(np.zeros((1, 2, 640), np.float32))
+    table, starts = leaf(np.arange(40, dtype=np.int32)[None]), leaf(np.array([0, 30], np.int32))
+    k, q = leaf(g.standard_normal((30, 128)).astype(np.float16)), leaf(g.standard_normal((30, 4, 64)).astype(np.float16))
+    waiting, used = None, []
+    for step in range(20):
+        after = k.paged_append(k, nn.PagedState(keys, values, table, starts, leaf(np.array([30 * (step + 1)], np.int32)), mass))
+        out = q.paged_attention(after, 0.125)
+        if waiting is not None:
+            assert np.isfinite(waiting.to_numpy()).all()
+        waiting = out
+        del after, out
+        dev.sync()
+        used.append(dev.pool_stats()[0])
+    assert len(set(used[3:])) == 1
+    assert np.isfinite(waiting.to_numpy()).all()
+
+
 @pytest.mark.parametrize("dt", [F16, F32])
 def test_rotary_axes_of_the_graph(dev, dt):
     """Positions per token through the lazy graph, into a paged cache."""

@@ -92,6 +92,74 @@ def test_builders_refuse_what_does_not_fit():
     assert axes(2, 2, 64, 0, leaf(I32, 2, 4), sec(10, 6)) == capi.ERR_INVALID_ARG
 
 
+def test_nodes_over_a_cache_run_in_the_order_in_which_they_were_built():
+    """An eviction behind an attention whose weights it goes by, though it takes the lengths of the append before; an append behind both; not behind nodes over other
+    pages, nor behind one that was released."""
+    from ratchet_b200 import capi
+    lib, F16, I32, F32 = capi.lib(), capi.F16, capi.I32, capi.F32
+    room = iter(range(1, 1000))
+
+    def leaf(dt, *shape):
+        t = capi.describe(dt, shape, next(room) << 20)       # a place of its own: what overlaps is what the same tensor holds
+        h = C.c_void_p()
+        assert lib.rcu_lazy_wrap(None, C.byref(t), C.byref(h)) == capi.OK
+        return h
+
+    def order(node):
+        n, ids = C.c_uint32(), (C.c_uint64 * 64)()
+        assert lib.rcu_lazy_execution_order(node, ids, 64, C.byref(n)) == capi.OK
+        return [ids[i] for i in range(n.value)]
+
+    def made(call, *args):
+        out = C.c_void_p()
+        assert call(*args, C.byref(out)) == capi.OK
+        return out
+
+    ident = lib.rcu_lazy_id
+    table, starts, lengths = leaf(I32, 3, 2), leaf(I32, 4), leaf(I32, 3)
+    k, q = leaf(F16, 5, 128), leaf(F16, 5, 4, 64)
+    caches = [(leaf(F16, 4, 2, 16, 64), leaf(F16, 4, 2, 16, 64), leaf(F32, 3, 2, 32)) for _ in range(2)]
+
+    def append(c, lengths, mass=True):
+        return made(lib.rcu_lazy_paged_append, k, 0, k, 0, c[0], c[1], table, starts, lengths, c[2] if mass else None)
+
+    def attend(c, lengths, mass=True):
+        return made(lib.rcu_lazy_paged_attention, q, c[0], c[1], table, starts, lengths, c[2] if mass else None, None, 0, 0, 0.1)
+
+    def evict(c, lengths, into):
+        return made(lib.rcu_lazy_paged_evict, c[0], c[1], table, lengths, c[2], into[0], into[1], table, into[2], 8, 2, 6)
+
+    c, other = caches
+    a = append(c, lengths)
+    dropped = attend(c, a)
+    gone = ident(dropped)
+    lib.rcu_lazy_release(dropped)
+    at = attend(c, a)
+    plain = attend(c, a, mass=False)                         # reads pages alone
+    elsewhere = append(other, lengths)
+    e = evict(c, a, c)
+    got = order(e)
+    assert gone not in got and ident(elsewhere) not in got
+    assert got[-1] == ident(e) and got.index(ident(a)) < got.index(ident(at)) and got.index(ident(a)) < got.index(ident(plain))
+    # reading orders nothing: two attentions, one of them with sums, only come after the append
+    assert ident(at) not in order(plain) and order(at)[-1] == ident(at)
+    # a step later: an append behind the eviction and all before it, the next attention behind that; into other pages one that does not write the old ones
+    a2 = append(c, e)
+    at2 = attend(c, a2)
+    assert [i for i in order(at2) if i in {ident(x) for x in (a, at, plain, e, a2, at2)}][-3:] == [ident(e), ident(a2), ident(at2)]
+    e2 = evict(c, a2, other)
+    assert {ident(at2), ident(elsewhere)} <= set(order(e2))
+    # the same tensors through a view
+    shape = (C.c_uint64 * 4)(4, 2, 16, 64)
+    views = [made(lib.rcu_lazy_view, x, 4, shape) for x in c[:2]] + [c[2]]
+    assert ident(at2) in order(evict(views, lengths, views))
+    # a handle that goes away while a later node holds its node
+    lib.rcu_lazy_release(at2)
+    assert order(e2)[-1] == ident(e2)
+    for h in (e2, a2, e, elsewhere, plain, at, a):
+        lib.rcu_lazy_release(h)
+
+
 # ---------------------------------------------------------------------------------------- handles
 class Pool:
     """A device's part in a buffer's life."""
