@@ -279,6 +279,34 @@ def test_attention_under_a_row_far_above_all_others(dev, dt, n, L):
 
 
 @pytest.mark.parametrize("dt", DTS)
+def test_single_weights_keep_their_bits(dev, dt):
+    """One query of 32 heads, each with two rows of weight: row 0, and one of its own whose sum is then that one weight e^-d / (1 + e^-d).  Scores are exact.  In
+    units of log 2 the exponent is off by log2 e's rounding (d log2 e < 2.9: 1.8e-7), its own (1.2e-7), and the lse's: the other weight's exponential (2^-22 of at
+    most half the sum), the product's and the sum's roundings (3e-7 together), log2f's last place (4.8e-7 in f16, where the sum is 128 times as large); times
+    ln 2 that is 7.5e-7 of the weight.  Its own exponential adds 2^-22."""
+    H = D = 32
+    c = pp.Cache(rng(1), dt, [1], [130], 1, D, D, 16)
+    d = (np.arange(4 * H).reshape(4, H) + 1) / 64
+    for turn in range(4):
+        k = np.full((130, D), -200.0)
+        k[0] = 0
+        own = 3 * np.arange(H) + 5 + turn
+        k[own, np.arange(H)] = -d[turn]
+        keys = pp.decode(c.keys, dt)
+        for r in range(130):
+            keys[c.table[0, r // 16], 0, r % 16] = k[r]
+        c.keys = pp.encode(keys, dt)[0]
+        q = put(dev, np.eye(H)[None], dt)[0]
+        cache = device_cache(dev, c, np.zeros((1, 1, c.rows)))
+        dev.paged_attention(q, cache, 1.0)
+        got = cache.mass.to_numpy()[0, 0].astype(np.float64)
+        want = np.exp(-d[turn]) / (1 + np.exp(-d[turn]))
+        assert np.abs(got[own] / want - 1).max() <= 1.0e-6
+        others = np.delete(got, np.concatenate([[0], own]))
+        assert not others.any() and abs(got[0] - (H - want.sum())) < 1e-5
+
+
+@pytest.mark.parametrize("dt", DTS)
 def test_attention_leaves_rows_of_no_sequence(dev, dt):
     g = rng(11)
     c = pp.Cache(g, dt, [3, 5], [30, 5], 2, 64, 64, 16)
