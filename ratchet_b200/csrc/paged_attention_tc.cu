@@ -505,8 +505,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                 const int h = seg.g * x.group + head, part_row = (two ? w : 0) * kTileQ + r;
                 float inv = scale0;
                 if (seg.whole) {
-                    if (a.sink && valid) l += ex2(a.sink[h] * kLog2e - m);
-                    const float f = valid && row >= 0 ? 1.f / l : 0.f;
+                    float f = 1.f;
+                    if (a.sink && valid) {          // against the larger one: the maximum may be minus infinity
+                        const float sk = a.sink[h] * kLog2e, top = fmaxf(m, sk);
+                        f = ex2(m - top);
+                        l = l * f + ex2(sk - top);
+                        m = top;
+                    }
+                    f = valid && row >= 0 ? f / l : 0.f;
                     inv *= f;
                     scale1 *= f;
                     if (a.lse && valid) a.lse[(size_t)(it.token + token) * a.H + h] = m + log2f(l);

@@ -254,6 +254,31 @@ def test_a_token_without_a_softmax_has_no_part_in_the_sums_of_rows_that_it_does_
     dev.sync()
 
 
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("n,L,D,window", [(70, 300, 64, 25), (200, 200, 80, 40), (4, 60, 64, 3), (9, 40, 136, 4), (40, 40, 64, 0)])
+def test_a_sink_beside_nothing_but_minus_infinities(dev, dt, n, L, D, window):
+    """A token that has minus infinity for every row that it sees gives all its weight to the sink: its output is zero, and no row's sum grows by it."""
+    g = rng(n + L + 1)
+    H, G, upto = 4, 2, L - n + n // 3 + 1
+    c = pp.Cache(g, dt, [n], [L], G, D, D, 16)
+    q = g.standard_normal((n, H, D))
+    q[:, :, 0] = 1.0
+    keys = pp.decode(c.keys, dt)
+    for r in range(upto):
+        c.k[0][r, 1, 0] = keys[c.table[0, r // 16], 1, r % 16, 0] = -np.inf
+    c.keys = pp.encode(keys, dt)[0]
+    q, qv = put(dev, q, dt)
+    sink = np.array([0.5, -30.0, 2.0, -1.0], np.float32)
+    want, size, mass = pp.attention(c, qv, 0.125, sink, window)
+    assert np.isfinite(want).all() and np.isfinite(mass[0]).all() and not want[0, 2:].any()
+    d = device_cache(dev, c, np.zeros((1, G, c.rows)))
+    got = get(dev.paged_attention(q, d, 0.125, up(dev, sink), window)).reshape(n, H, D)
+    assert close(got, want, size, dt, 5.0) and not got[0, 2:].any()
+    grown = d.mass.to_numpy()[0, :, :L].astype(np.float64)
+    assert np.all(np.abs(grown - mass[0]) <= 2e-5 * mass[0] + 4 * 2.0 ** -24 * (1 + mass[0]))
+    dev.sync()
+
+
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("n,L", [(1, 131000), (8, 20008), (64, 20064)])
 def test_attention_under_a_row_far_above_all_others(dev, dt, n, L):
