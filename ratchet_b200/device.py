@@ -19,7 +19,7 @@ from .capi import RatchetCudaError
 class Buffer:
     """A resolved tensor on the device: dtype, logical shape and one pooled allocation."""
 
-    __slots__ = ("dev", "dt", "shape", "ptr", "nbytes", "_owned", "_base", "_byref")
+    __slots__ = ("dev", "dt", "shape", "ptr", "nbytes", "_owned", "_base", "_byref", "_described")
 
     def __init__(self, dev: "Device", dt: int, shape, ptr: int, nbytes: int, owned: bool, base=None):
         self.dev = dev
@@ -29,7 +29,7 @@ class Buffer:
         self.nbytes = nbytes
         self._owned = owned
         self._base = base  # keeps the owning buffer alive for views
-        self._byref = None  # reference to a descriptor, made by the first call that takes this buffer
+        self._byref = self._described = None  # reference to a descriptor, and what that says
 
     @property
     def numel(self) -> int:
@@ -40,6 +40,13 @@ class Buffer:
 
     def desc(self) -> capi.rcu_tensor:
         return capi.describe(self.dt, self.shape, self.ptr)
+
+    def ref(self):
+        """A descriptor for the C ABI, which only reads it.  Kept as long as it is true: making one takes longer than a short kernel runs."""
+        now = (self.ptr, self.dt, tuple(self.shape))
+        if now != self._described:
+            self._byref, self._described = C.byref(self.desc()), now
+        return self._byref
 
     def view(self, shape) -> "Buffer":
         """Same storage, new shape (Tensor::view, tensor.rs:454-461)."""
@@ -65,7 +72,6 @@ class Buffer:
             self.dev._free(self.ptr)
             self.ptr = 0
             self._owned = False
-            self._byref = None
 
     def __del__(self):
         try:
@@ -81,21 +87,19 @@ class PagedCache:
 
     def __init__(self, keys: Buffer, values: Buffer, table: Buffer, lengths: Buffer, starts: Optional[Buffer] = None, mass: Optional[Buffer] = None):
         self.keys, self.values, self.table, self.starts, self.lengths, self.mass = keys, values, table, starts, lengths, mass
-        self._named = self._owners = self._ref = None
+        self._refs = self._ref = None
 
     @property
     def ref(self):
         """The descriptor for the C ABI, of the buffers as they are now: one that was put in another's place counts, and one that was freed is refused (a
         structure made earlier would still name its block, which the pool may have handed on)."""
-        named = (self.keys, self.values, self.table, self.starts, self.lengths, self.mass)
-        if named != self._named or not all([b.ptr for b in self._owners]):
-            owners = [b._base or b for b in named if b is not None]
-            for b in owners:
-                if not b.ptr:
-                    self._named = None
-                    raise RatchetCudaError(capi.ERR_INVALID_ARG, "paged cache: a buffer of it has been freed")
-            self._ref = C.byref(capi.rcu_paged(*(capi.rcu_tensor() if b is None else b.desc() for b in named)))
-            self._named, self._owners = named, owners
+        refs = []
+        for b in (self.keys, self.values, self.table, self.starts, self.lengths, self.mass):
+            if b is not None and not (b._base or b).ptr:
+                raise RatchetCudaError(capi.ERR_INVALID_ARG, "paged cache: a buffer of it has been freed")
+            refs.append(None if b is None else b.ref())
+        if refs != self._refs:                              # kept references: a descriptor that has changed is another object
+            self._ref, self._refs = C.byref(capi.rcu_paged(*(capi.rcu_tensor() if r is None else r._obj for r in refs))), refs
         return self._ref
 
     @property
@@ -212,12 +216,7 @@ class Device:
 
     # ------------------------------------------------------------------ ops (eager, one C-ABI call each)
     def _ref(self, b: Optional[Buffer]):
-        """A descriptor of the buffer for the C ABI, which only reads it.  Kept by the buffer: making one takes longer than a short kernel runs."""
-        if b is None:
-            return None
-        if b._byref is None:
-            b._byref = C.byref(b.desc())
-        return b._byref
+        return None if b is None else b.ref()
 
     def dequantize(self, src: Buffer, out: Optional[Buffer] = None) -> Buffer:
         out = out or self.empty(capi.activation_dtype(src.dt), src.shape)

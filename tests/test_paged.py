@@ -201,6 +201,27 @@ def test_a_cache_names_its_buffers_as_they_are(name, view):
         PagedCache(**{n: made.get(n) for n in shapes}).ref
 
 
+def test_descriptors_say_what_their_buffers_do():
+    """Calls keep a buffer's descriptor as long as its address, type and shape are the ones it has."""
+    from ratchet_b200 import Buffer, PagedCache, capi
+    from ratchet_b200.device import Device
+    call = Device._ref                                      # what every call makes of a buffer
+    b = Buffer(None, capi.F16, (4, 2, 16, 64), 0x1000, 64, False)
+    rest = [Buffer(None, t, s, 0x2000, 64, False) for t, s in ((capi.F16, (4, 2, 16, 64)), (capi.I32, (2, 2)), (capi.I32, (2,)))]
+    c = PagedCache(b, *rest)
+    assert call(None, None) is None and call(None, b) is call(None, b) and c.ref is c.ref
+    b.ptr = 0x5000
+    assert call(None, b)._obj.data == 0x5000 == c.struct.keys.data
+    b.shape = (8, 2, 16, 32)
+    assert list(call(None, b)._obj.shape) == [8, 2, 16, 32] == list(c.struct.keys.shape)
+    b.dt = capi.BF16
+    assert call(None, b)._obj.dt == capi.BF16 == c.struct.keys.dt
+    b.shape = [8, 2, 16, 32]
+    call(None, b)
+    b.shape[0] = 3
+    assert call(None, b)._obj.shape[0] == 3
+
+
 def test_a_cache_without_starts_and_sums():
     from ratchet_b200 import Buffer, PagedCache, capi
     b = lambda dt, *s: Buffer(None, dt, s, 0x1000, 64, False)  # noqa: E731
