@@ -152,7 +152,7 @@ void order_paged(rcu_lazy* n) {
     PagedNodes& all = paged_nodes();
     n->own = n->srcs.size();
     const std::lock_guard<std::mutex> lock(all.mutex);
-    all.nodes.erase(std::remove_if(all.nodes.begin(), all.nodes.end(), [](const rcu_lazy* t) { return t->resolved(); }), all.nodes.end());
+    all.nodes.erase(std::remove_if(all.nodes.begin(), all.nodes.end(), [n](const rcu_lazy* t) { return t->dev == n->dev && t->resolved(); }), all.nodes.end());          // another device's may be resolving
     for (rcu_lazy* t : all.nodes) {
         if (t->dev != n->dev || std::find(n->srcs.begin(), n->srcs.end(), t) != n->srcs.end() || !follows(t, n)) continue;
         uint32_t refs = t->refs.load(std::memory_order_relaxed);
