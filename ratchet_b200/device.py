@@ -80,6 +80,9 @@ class Buffer:
             pass
 
 
+_ABSENT = Buffer(None, 0, (1,), -1, 0, False)               # in the place of a buffer that a cache has not
+
+
 class PagedCache:
     """``rcu_paged`` over device buffers: pages of keys and values [pages, kv_heads, page_rows, features], the table I32 [sequences, max_pages],
     starts I32 [sequences + 1] of a call's new tokens, lengths I32 [sequences] with them, and (optional) the attention weight F32
@@ -87,19 +90,23 @@ class PagedCache:
 
     def __init__(self, keys: Buffer, values: Buffer, table: Buffer, lengths: Buffer, starts: Optional[Buffer] = None, mass: Optional[Buffer] = None):
         self.keys, self.values, self.table, self.starts, self.lengths, self.mass = keys, values, table, starts, lengths, mass
-        self._refs = self._ref = None
+        self._now = self._ref = None
+        self._bases = ()
 
     @property
     def ref(self):
         """The descriptor for the C ABI, of the buffers as they are now: one that was put in another's place counts, and one that was freed is refused (a
-        structure made earlier would still name its block, which the pool may have handed on)."""
-        refs = []
-        for b in (self.keys, self.values, self.table, self.starts, self.lengths, self.mass):
-            if b is not None and not (b._base or b).ptr:
+        structure made earlier would still name its block, which the pool may have handed on).  Asked for in every call: kept while nothing changes."""
+        k, v, t, n, s, m = self.keys, self.values, self.table, self.lengths, self.starts or _ABSENT, self.mass or _ABSENT
+        now = (k.ptr, k.shape, k.dt, v.ptr, v.shape, v.dt, t.ptr, t.shape, t.dt, n.ptr, n.shape, n.dt, s.ptr, s.shape, s.dt, m.ptr, m.shape, m.dt)
+        if now != self._now or self._bases and not all([b.ptr for b in self._bases]):
+            named = [k, v, t, None if s is _ABSENT else s, n, None if m is _ABSENT else m]
+            self._now = None
+            if not all([(b._base or b).ptr for b in named if b is not None]):
                 raise RatchetCudaError(capi.ERR_INVALID_ARG, "paged cache: a buffer of it has been freed")
-            refs.append(None if b is None else b.ref())
-        if refs != self._refs:                              # kept references: a descriptor that has changed is another object
-            self._ref, self._refs = C.byref(capi.rcu_paged(*(capi.rcu_tensor() if r is None else r._obj for r in refs))), refs
+            self._ref = C.byref(capi.rcu_paged(*(capi.rcu_tensor() if b is None else b.desc() for b in named)))
+            self._bases = tuple([b._base for b in named if b is not None and b._base is not None])
+            self._now = now
         return self._ref
 
     @property
@@ -216,7 +223,9 @@ class Device:
 
     # ------------------------------------------------------------------ ops (eager, one C-ABI call each)
     def _ref(self, b: Optional[Buffer]):
-        return None if b is None else b.ref()
+        if b is None:
+            return None
+        return b._byref if b._described == (b.ptr, b.dt, tuple(b.shape)) else b.ref()
 
     def dequantize(self, src: Buffer, out: Optional[Buffer] = None) -> Buffer:
         out = out or self.empty(capi.activation_dtype(src.dt), src.shape)
