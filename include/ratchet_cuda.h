@@ -316,13 +316,14 @@ typedef struct {
 rcu_status rcu_rotary_axes(rcu_device* dev, const rcu_tensor* x, uint32_t x_col, uint32_t first, const rcu_tensor* freqs, float magnitude,
                            const rcu_tensor* positions, const uint32_t* sections, int halves, rcu_tensor* dst);
 /* Keys (columns [k_col, k_col + kv_heads * dim) of the rows k) and values (of the rows v, which may be k) of the new tokens into their pages; the
- * rows' mass, where it is kept, becomes zero.  Two tokens of one call must not go to the same row of a page. */
+ * rows' mass, where it is kept, becomes zero.  Two tokens of one call must not go to the same row of a page, nor may k or v lie in rows that the call writes. */
 rcu_status rcu_paged_append(rcu_device* dev, const rcu_tensor* k, uint32_t k_col, const rcu_tensor* v, uint32_t v_col, const rcu_paged* cache);
 /* Softmax attention of the new tokens (already appended) over their sequences' pages: q [tokens, H, dim], query head h reads key / value head
  * h / (H / kv_heads).  The token at row r of its sequence sees rows j <= r, with window > 0 only those with j > r - window or j < first.
  * sink F32 [H] (nullable): exp(sink[h]) joins the denominator.  dst [tokens, H * vdim].  Where mass is kept, every row's sum grows by the
  * weights (shares of the denominator) that the group's heads and the new tokens give it; sums are formed in the same order in every call.
- * dst must not overlap q.  With mass, sequences * kv_heads are 65535 at most.
+ * In F16 and BF16 a weight may be rounded to that type before it meets the values; the sums of weights, and the weights that rows receive, are of 32 bits.
+ * dst must not overlap q, nor anything else that the call reads or writes.  With mass, sequences * kv_heads are 65535 at most.
  * scratch (nullable): device memory of rcu_paged_attention_scratch bytes on a 256-byte boundary, any dtype; NULL takes it from the pool, which is
  * refused while the stream is being captured.  Calls that share a scratch must not overlap. */
 rcu_status rcu_paged_attention(rcu_device* dev, const rcu_tensor* q, const rcu_paged* cache, const rcu_tensor* sink, uint32_t window, uint32_t first,

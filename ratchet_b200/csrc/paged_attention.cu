@@ -10,7 +10,8 @@ namespace {
 
 using namespace paged;
 
-// A warp per token and head.
+// A warp per token and head, for what the other two kernels do not take; a lane reads keys element by element.  64 sequences of 4000 rows, 32 heads over 8 of 192
+// features, bf16: 14.8 ms (of 128 features, on the other path, 0.19); a prompt of 1024 tokens 17.0 ms (0.05).
 template <class T>
 __global__ void __launch_bounds__(128) attend_kernel(const AttendArgs a) {
     rcu_kernel_entry();

@@ -1,14 +1,14 @@
 // Attention of few new tokens over paged caches: generation in f16 and bf16, and f32 of any length.  Heads of up to 128 features.
 //
 // An item is up to 16 (f32: 8) rows of queries - tokens with the heads of a group, one after the other - and a warp takes slices of 16 cached rows,
-// which lie in one page, by itself: it asks for them by TMA into a ring of its own, three slices deep, works out scores, weights and sums in
-// registers, and meets the other warps only at the end of the item's part, where their maxima and sums are joined.  Nothing in between waits for
+// which lie in one page, by itself: it asks for them by TMA into a ring of its own, three slices deep (f32: one to three, launch_rows), works out scores, weights and
+// sums in registers, and meets the other warps only at the end of the item's part, where their maxima and sums are joined.  Nothing in between waits for
 // another warp, so what bounds it is the memory: 64 bytes a row and feature pair are in flight on every SM all the time.
 //   f16, bf16   both products by mma.sync m16n8k16: 16 rows do not fill a tile of the 5th-generation tensor cores, whose turn-around through tensor
 //               memory took 2500 cycles for 128 rows here (tensor memory, softmax of one warp, tensor memory again) against 1300 that the memory needs;
 //   f32         FMA: a lane has a cached row and four queries for the scores, four features of the values and all queries for the sum; bound by the chain of a
 //               slice in a warp (1600 instructions with eight queries, two warps a scheduler, 45 % of the issue slots).
-// 64 sequences of 100 to 8000 rows, 32 heads over 8, 128 features: bf16 184 us of 164 that the memory needs (5.8 TB/s); f32 403 us (5.3 TB/s).
+// 64 sequences of 100 to 8000 rows, 32 heads over 8, 128 features: bf16 191 us of 164 that the memory needs (5.6 TB/s), f16 the same; f32 402 us (5.3 TB/s).
 // One token of one sequence of 1000 rows, 32 heads of 96 features: 15.3 us, of which the attention 11: items, then a chain of three slices, then the joins.
 // Weights are rounded to the operands' type for the second product and taken against the maximum less 7 in f16, as in paged_attention_tc.cu; values that are masked and not
 // finite are kept out the same way.  Every wait is bounded; a warp whose wait gave up goes through the motions, so that the CTA's barriers are met.
@@ -579,9 +579,13 @@ bool attend_rows_takes(const rcu_device* dev, const View& p, int H, int dt) {
     // This kernel against the tensor cores', 64 sequences of up to 8000 rows, 8 kv heads: 8 rows 189 us / 213, 16 rows 201 / 228, 32 rows 380 / 225;
     // up to 500 rows long: 16 rows 53 / 66, 32 rows 84 / 55; one sequence of 131000: 16 rows 105 / 120, 32 rows 182 / 120; one of 1000 rows: 16 rows 18.0 / 22.0,
     // 32 rows 18.5 / 21.3 (the only place on the far side where this one leads).
+    // All of these have sequences that bring the same; what the average hides is dear: one chunk of 769 tokens behind 16000 rows among 255 single tokens behind 500, four
+    // heads a group, takes 2640 us here, where the chunk by itself takes 251 and the others 154 (65 tokens behind 131000 rows, eight heads: 2734 and 418).
     if (dt != RCU_F32 && (uint64_t)p.T * group > 16ull * p.S) return false;
     if (((uint64_t)p.T * group / 8 + p.S) * (((uint64_t)p.MP << p.shift) / kTileK + 2) * p.G >= (1ull << 31)) return false;
-    return !p.mass || (uint64_t)p.T * H * ((uint64_t)p.MP << p.shift) <= (1ull << 27);          // the scores: half a GB
+    // The scores: half a GB, by the table's width, since the host knows no lengths.  f32 beyond it has the plain kernels alone: 64 sequences of 500 rows, 32 heads over 8,
+    // 64 features, in tables of 65536 rows 107 us, of 131072 rows 1431.
+    return !p.mass || (uint64_t)p.T * H * ((uint64_t)p.MP << p.shift) <= (1ull << 27);
 }
 
 uint64_t attend_rows_scratch(const rcu_device* dev, const View& p, int H, int dt) { return rows_plan_of(dev, p, H, dt, nullptr, nullptr, nullptr); }

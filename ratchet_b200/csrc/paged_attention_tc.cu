@@ -17,9 +17,9 @@
 // shared memory.  In a tile that some of the queries see in part, an infinity or NaN among the values sends the query tile to attend_rows, which
 // reads only what each query sees.
 // Every wait is bounded; one that gives up raises RCU_DEVFLAG_TIMEOUT and ends all others of the CTA.
-// Bound by the softmax warps' chains (two of them a scheduler): 4096 tokens into an empty cache, 32 heads over 8 of 128 features, bf16: 184 us (750 TFLOP/s; tensor
-// pipe 40 %, exponentials 30 %, issue slots 40 %); 777 tokens over 20000 rows, 80 features, f16: 283 us.  With two threads a query 229 and 365 us: what they have to tell
-// each other costs more than the shorter chains gain.  With a whole warp keeping step with the issuing lane 184 and 291.
+// Bound by the softmax warps' chains (two of them a scheduler): 4096 tokens into an empty cache, 32 heads over 8 of 128 features, bf16: 196 us (700 TFLOP/s; 189 in passes
+// right behind one another; tensor pipe 40 %, exponentials 30 %, issue slots 44 %); 777 tokens over 20000 rows, 80 features, f16: 288 us.  Two threads a query had taken
+// 229 us for 184 and 365 for 283: what they have to tell each other costs more than the shorter chains gain.  A whole warp keeping step with the issuing lane 291 for 283.
 #include <cuda.h>
 
 #include "paged_attention.cuh"

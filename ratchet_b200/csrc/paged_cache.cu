@@ -126,7 +126,8 @@ void launch_append(rcu_device* dev, const View& p, const void* k, uint64_t k_pit
 //      place is never behind its old one, so what a round writes has been read in it or before.  Into other arrays: a kernel behind this one, in
 //      which nobody waits (in rounds the copy of 4096 rows of 16 sequences by 8 heads took 130 us, 4.1 TB/s).
 // Bound by memory: the masses, then 2 keep (D + E) elements.  4096 of up to 16000 rows, 16 sequences, 8 heads, bf16, 128 features: 132 us, of which the selection 40 (four
-// passes with a barrier of the cluster each), the copy 92 at 6.0 TB/s; 1000 of 2048 rows of one sequence 17.8 us.
+// passes with a barrier of the cluster each), the copy 92 at 6.0 TB/s; 1000 of 2048 rows of one sequence 18.6 us.  In place, where the copy goes in rounds: 220 us for 132.
+// 64 registers a thread keep four CTAs on an SM and spill 40 bytes.
 constexpr int kEvictThreads = 256, kEvictUnits = 8, kEvictCluster = 8, kEvictCodes = 6144;
 
 struct EvictArgs {

@@ -10,7 +10,7 @@
 //   warp 1            S^T of every query tile, four buffers of tensor memory;
 //   warps 2-5, 6-9    every other query tile each: exponentials and sums, which are joined at the end of the item.
 // Bound by the exponentials and what is issued around them: 128 x 128 of them take 1024 cycles of an SM, the product half of that.  777 tokens over 20000 rows,
-// 32 heads over 8, 80 features: 196 us (exponential pipe 51 %, issue slots 42 %, tensor pipe 21 %).
+// 32 heads over 8, 80 features: 193 us (exponential pipe 52 %, issue slots 49 %, tensor pipe 21 %).
 // Every wait is bounded; one that gives up raises RCU_DEVFLAG_TIMEOUT and ends all others of the CTA.
 #include "paged_tc.cuh"
 

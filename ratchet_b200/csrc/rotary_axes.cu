@@ -5,8 +5,9 @@
 //
 // Bound by memory: every row is read and written once.  A CTA takes a few tokens: it works out their angles once, in shared memory, and then
 // turns all their heads, sixteen bytes of a row per thread and step.  The angle is a product of doubles, brought into [-pi, pi] by doubles
-// (so positions of any size keep their low bits), and only there goes on in f32: sine and cosine of a reduced f32 are off by
-// 1.2e-7 at most, half a unit of f32, and cost a tenth of a double's.  8192 tokens, 16 heads of 128, three axes, f16: 16.2 us (4.1 TB/s); 32 tokens 4.9 us.
+// (so positions of any size keep their low bits), and only there goes on in f32, which costs a tenth of a double's sine: its rounding moves the angle by 2^-23
+// (1.2e-7) at most, and sincosf's results are off by two units in the last place at most (1.2e-7 again).  The table's two floats leave 2^-48 of the angle open.
+// 8192 tokens, 16 heads of 128, three axes, f16: 20.5 us (3.3 TB/s), 17 where the passes before have left the rows in L2; 32 tokens 5.1 us.
 #include "lm_math.cuh"
 
 namespace {
@@ -32,7 +33,7 @@ __device__ __forceinline__ float2 turn_of(const AxesArgs& a, long long t, int i)
     return make_float2(c * a.magnitude, s * a.magnitude);
 }
 
-// V elements of 16 bytes (VEC), or one by one; TOK tokens per CTA
+// V elements of 16 bytes (VEC), or one by one; `tokens` tokens per CTA
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) rotary_axes_kernel(const AxesArgs a, const T* x, T* out, int tokens, int ahead) {
     rcu_kernel_entry();
@@ -50,7 +51,7 @@ __global__ void __launch_bounds__(256) rotary_axes_kernel(const AxesArgs a, cons
     if constexpr (VEC) {
         constexpr int V = 16 / (int)sizeof(T);
         struct alignas(16) Vec { T v[V]; };
-        // a thread has one place of a row, in every token or every few, and asks for several tokens at once
+        // a thread has one place of a row, in every token or every few, one after the other: dst may be x itself, so no token is read ahead of the one before
         const int places = a.H * (a.halves ? a.pairs / V + (a.D - 2 * a.pairs) / V : a.D / V), abreast = max(1, 256 / places);
         const int first_place = places < 256 ? (int)threadIdx.x % places : (int)threadIdx.x, first_token = places < 256 ? (int)threadIdx.x / places : 0;
         if (first_token >= abreast) return;
@@ -134,7 +135,8 @@ template <class T> void launch_axes(rcu_device* dev, const AxesArgs& a, const vo
     const unsigned grid = (unsigned)((a.T + tokens - 1) / tokens);
     const size_t smem = (size_t)tokens * a.pairs * sizeof(float2);
     // Rows are asked for ahead of the angles where x and dst together are larger than L2, so that x comes from memory: 8192 tokens, 32 heads of 128 in f32 50.4 -> 43.4 us;
-    // with half the heads in f16, which stay in L2, the requests cost 16.4 -> 17.2
+    // with half the heads in f16, which stay in L2 from one such pass to the next, the requests cost 16.4 -> 17.2.  Where other work has put smaller rows out of L2,
+    // nobody asks ahead, and the latter case takes 20.5
     const int ahead = 2 * a.T * a.H * a.D * (long long)sizeof(T) > (126ll << 20);
     if (vec) rcu_launch(dev, rotary_axes_kernel<T, true>, grid, 256, smem, a, (const T*)x, (T*)out, tokens, ahead);
     else rcu_launch(dev, rotary_axes_kernel<T, false>, grid, 256, smem, a, (const T*)x, (T*)out, tokens, ahead);
