@@ -98,7 +98,7 @@ class PagedCache:
         """The descriptor for the C ABI, of the buffers as they are now: one that was put in another's place counts, and one that was freed is refused (a
         structure made earlier would still name its block, which the pool may have handed on).  Asked for in every call: kept while nothing changes."""
         k, v, t, n, s, m = self.keys, self.values, self.table, self.lengths, self.starts or _ABSENT, self.mass or _ABSENT
-        now = (k.ptr, k.shape, k.dt, v.ptr, v.shape, v.dt, t.ptr, t.shape, t.dt, n.ptr, n.shape, n.dt, s.ptr, s.shape, s.dt, m.ptr, m.shape, m.dt)
+        now = (k, k.ptr, k.shape, k.dt, v, v.ptr, v.shape, v.dt, t, t.ptr, t.shape, t.dt, n, n.ptr, n.shape, n.dt, s, s.ptr, s.shape, s.dt, m, m.ptr, m.shape, m.dt)
         if now != self._now or self._bases and not all([b.ptr for b in self._bases]):
             named = [k, v, t, None if s is _ABSENT else s, n, None if m is _ABSENT else m]
             self._now = None

@@ -201,6 +201,21 @@ def test_a_cache_names_its_buffers_as_they_are(name, view):
         PagedCache(**{n: made.get(n) for n in shapes}).ref
 
 
+def test_a_cache_knows_whose_view_it_has():
+    """A view in the place of the buffer itself: the same address, but another's to free."""
+    from ratchet_b200 import Buffer, PagedCache, RatchetCudaError, capi
+    dev = Pool()
+    keys, values, table, lengths = (Buffer(dev, t, s, 0x1000 * i, 64, True) for i, (t, s) in enumerate(((capi.F16, (4, 2, 16, 64)), (capi.F16, (4, 2, 16, 64)), (capi.I32, (2, 2)),
+                                                                                                       (capi.I32, (2,))), 1))
+    c = PagedCache(keys, values, table, lengths)
+    c.ref
+    c.keys = keys.view(keys.shape)
+    assert c.struct.keys.data == 0x1000
+    keys.free()
+    with pytest.raises(RatchetCudaError):
+        c.ref
+
+
 def test_descriptors_say_what_their_buffers_do():
     """Calls keep a buffer's descriptor as long as its address, type and shape are the ones it has."""
     from ratchet_b200 import Buffer, PagedCache, capi
